@@ -13,11 +13,16 @@ LB_OK = 0
 LB_E_ARG, LB_E_ALIGN, LB_E_DEVICE, LB_E_LAUNCH, LB_E_WORKSPACE, LB_E_UNSUPPORTED = -1, -2, -3, -4, -5, -6
 FMT_INT8_ROW, FMT_INT4_G128, FMT_Q8_0_G32, FMT_Q4_0_G32 = 1, 2, 3, 4
 FMT_FP8_E4M3, FMT_FP8_E5M2, FMT_FP6_E3M2, FMT_FP6_E2M3, FMT_FP4_E2M1 = 5, 6, 7, 8, 9
+FMT_MXFP4, FMT_NVFP4 = 10, 11
+MICROSCALED_FMT = {"mxfp4": FMT_MXFP4, "nvfp4": FMT_NVFP4}
+MX_MAX_GROUPS = 1024
+MX_PARTIALS = 1023
 MINIFLOAT_FMT = {"fp8_e4m3": FMT_FP8_E4M3, "fp8_e5m2": FMT_FP8_E5M2, "fp6_e3m2": FMT_FP6_E3M2,
                  "fp6_e2m3": FMT_FP6_E2M3, "fp4_e2m1": FMT_FP4_E2M1}
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 DEVERR_WAIT_TIMEOUT = 1
 DEVERR_PEER_TIMEOUT = 2
+DEVERR_BAD_INDEX = 4
 IPC_HANDLE_BYTES = 64
 MAX_RANKS = 8
 LINEAR_STATIC_WEIGHTS = 1
@@ -66,6 +71,16 @@ SIGNATURES = [
     ("lb_qkv_prep", _I, [_P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _P, _I64, _P, _I64, _I64, _I64,
                          _P, _P, _I64, _I64, _P]),
     ("lb_act_mul", _I, [_P, _I64, _I64, _I, _P, _P]),
+    ("lb_mx_row_bytes", _I64, [_I64]),
+    ("lb_mx_scale_bytes", _I64, [_I, _I64, _I64, _I64, _I64]),
+    ("lb_mx_quant", _I, [_I, _P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P]),
+    ("lb_mx_dequant", _I, [_I, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I, _I64, _P]),
+    ("lb_mx_scales", _I, [_I, _P, _I64, _I64, _I64, _I64, _P, _I, _P]),
+    ("lb_mx_linear", _I, [_I, _P, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I, _P, _I64, _P]),
+    ("lb_mx_linear_grouped", _I, [_I, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I, _P, _I64, _P]),
+    ("lb_moe_route_workspace_size", _I, [_I64, _I64, ctypes.POINTER(_SZ)]),
+    ("lb_moe_route", _I, [_P, _I, _I64, _I64, _I64, _I, _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    ("lb_moe_combine", _I, [_P, _I64, _I64, _P, _P, _I64, _I, _I64, _I, _P, _I64, _P]),
 ]
 
 

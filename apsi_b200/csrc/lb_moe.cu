@@ -1,0 +1,256 @@
+// The way to the experts and back.
+//
+//   route    p = softmax(logits[t, :]); the k largest of each token (equal logits: the lower index first), their
+//            weights (p, or p over the chosen ones' sum), and the T k rows in expert order (a stable counting
+//            sort of (token, j) by expert): offsets[E + 1], rows (the token of each place), slots (the place of each (t, j))
+//   combine  y[t, :] = sum_j weight[t, j] z[slots[t, j], :], float32, j in order
+//
+// Logits that are NaN count as -inf; an expert at -inf has weight 0 (a masked expert), and a token whose every
+// logit is -inf has weights 0.  +inf shares the weight evenly among the experts that have it.
+#include "lb_mx.cuh"
+#include "lb_kernels.h"
+
+namespace lb {
+namespace moe {
+
+constexpr int TOK = 64;                 // tokens of a chunk: one block ranks one chunk
+
+struct RouteParams {
+  const void* logits;
+  int dt;
+  int64_t ldl, T;
+  int E, k, normalize;
+  float* weights;
+  int* experts;
+  int* offsets;
+  int* rows;
+  int* slots;
+  int* counts;                          // [chunks][E]
+};
+
+__device__ __forceinline__ float logit(const RouteParams& p, int64_t t, int e) {
+  const int64_t i = t * p.ldl + e;
+  float v;
+  if (p.dt == LB_DT_F32) v = static_cast<const float*>(p.logits)[i];
+  else if (p.dt == LB_DT_BF16) v = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.logits)[i]) << 16);
+  else v = __half2float(static_cast<const __half*>(p.logits)[i]);
+  return v == v ? v : -INFINITY;
+}
+// float order as unsigned order (-0 and +0 are one value)
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// One warp per token: k rounds of a warp-wide maximum over what is left; L logits per lane.
+template <int L>
+__device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int* hist) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[L];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const int e = i * 32 + lane;
+    const float v = e < p.E ? logit(p, t, e) : -INFINITY;
+    key[i] = e < p.E ? order_key(v) : 0u;            // 0: none (every float's key is above it)
+    m = fmaxf(m, v);
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  auto weight = [&](uint32_t u) {
+    const float v = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+    return m == -INFINITY ? 0.f : (v == m ? 1.f : expf(v - m));
+  };
+  float sum = 0.f;
+  if (!p.normalize) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) if (key[i]) sum += weight(key[i]);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  float mine = 0.f;                                  // lane j holds choice j
+  int mine_e = 0;
+  for (int j = 0; j < p.k; ++j) {
+    uint32_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (key[i] > best) { best = key[i]; at = i; }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFFFFFu);
+    if ((e & 31u) == static_cast<uint32_t>(lane)) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) if (i == static_cast<int>(e >> 5)) key[i] = 0;
+    }
+    const float w = weight(top);
+    if (p.normalize) sum += w;
+    if (lane == j) { mine = w; mine_e = static_cast<int>(e); }
+  }
+  if (lane < p.k) {
+    p.weights[t * p.k + lane] = sum > 0.f ? mine / sum : 0.f;
+    p.experts[t * p.k + lane] = mine_e;
+    atomicAdd(&hist[mine_e], 1);                     // whole numbers: the order does not matter
+  }
+}
+
+// Chooses and counts: one block per chunk of TOK tokens.
+template <int L>
+__global__ void __launch_bounds__(256) route_choose_kernel(const RouteParams p) {
+  extern __shared__ int hist[];
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
+  __syncthreads();
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOK;
+  for (int i = threadIdx.x >> 5; i < TOK && t0 + i < p.T; i += blockDim.x >> 5) choose<L>(p, t0 + i, hist);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.E + e] = hist[e];
+}
+
+// Places: every block adds up the counts it needs, then one warp ranks its chunk's (token, j) in order.
+__global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p) {
+  extern __shared__ int next[];                      // [E] next free place of each expert for this chunk
+  __shared__ int carry;
+  const int chunks = gridDim.x;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    int before = 0, all = 0;
+    for (int c = 0; c < chunks; ++c) {
+      const int n = p.counts[static_cast<int64_t>(c) * p.E + e];
+      before += c < static_cast<int>(blockIdx.x) ? n : 0;
+      all += n;
+    }
+    next[e] = before;
+    next[p.E + e] = all;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {                            // exclusive scan over the experts
+    const int lane = threadIdx.x;
+    int run = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + lane;
+      const int n = e < p.E ? next[p.E + e] : 0;
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      if (e < p.E) {
+        next[e] += run + s - n;
+        if (blockIdx.x == 0) p.offsets[e] = run + s - n;
+      }
+      run += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (blockIdx.x == 0 && lane == 0) p.offsets[p.E] = run;
+    carry = 0;
+    __syncwarp();
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOK;
+    const int64_t left = p.T - t0;
+    const int n = static_cast<int>(left < TOK ? left : TOK) * p.k;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      const bool in = i < n;
+      const int e = in ? p.experts[t0 * p.k + i] : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, e);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int place = in ? next[e] + rank : 0;
+      __syncwarp();
+      if (in && rank == 0) next[e] += __popc(same);
+      __syncwarp();
+      if (in) {
+        p.slots[t0 * p.k + i] = place;
+        p.rows[place] = static_cast<int>(t0 + i / p.k);
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) combine_kernel(const uint16_t* __restrict__ z, int64_t ldz, int64_t rows,
+                                                      const float* __restrict__ w, const int* __restrict__ slots,
+                                                      int64_t T, int k, int64_t H, uint16_t* __restrict__ y, int64_t ldy,
+                                                      int acc) {
+  const int64_t total = T * H;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t t = i / H, h = i - t * H;
+    float s = acc ? __uint_as_float(static_cast<uint32_t>(y[t * ldy + h]) << 16) : 0.f;
+    for (int j = 0; j < k; ++j) {
+      const float wj = w[t * k + j];
+      const int r = slots[t * k + j];
+      if (r < 0 || r >= rows) {
+        atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
+        continue;
+      }
+      if (wj != 0.f) s = fmaf(wj, __uint_as_float(static_cast<uint32_t>(z[r * ldz + h]) << 16), s);
+    }
+    y[t * ldy + h] = f32_to_bf16_bits_g(s);
+  }
+}
+
+}  // namespace moe
+}  // namespace lb
+
+using namespace lb;
+
+extern "C" {
+
+int lb_moe_route_workspace_size(int64_t T, int64_t E, size_t* bytes) {
+  if (!bytes) return fail(LB_E_ARG, "lb_moe_route_workspace_size: bytes is NULL");
+  if (T < 0 || E <= 0) return fail(LB_E_ARG, "lb_moe_route_workspace_size: bad sizes");
+  *bytes = static_cast<size_t>((T + moe::TOK - 1) / moe::TOK) * E * sizeof(int);
+  return LB_OK;
+}
+
+int lb_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, int k, int normalize, float* weights,
+                 int* experts, int* offsets, int* rows, int* slots, void* workspace, size_t ws_bytes, void* stream) {
+  if (dtype != LB_DT_F32 && dtype != LB_DT_BF16 && dtype != LB_DT_F16)
+    return fail(LB_E_ARG, "lb_moe_route: dtype must be LB_DT_F32, LB_DT_BF16 or LB_DT_F16");
+  if (T < 0 || E <= 0 || E > LB_MX_MAX_GROUPS || ldl < E) return fail(LB_E_ARG, "lb_moe_route: E must be in [1, %d], ldl >= E", LB_MX_MAX_GROUPS);
+  if (k <= 0 || k > E || k > 32) return fail(LB_E_ARG, "lb_moe_route: k must be in [1, min(E, 32)]");
+  if (T * k > 0x7FFFFFFF) return fail(LB_E_ARG, "lb_moe_route: T k must be below 2^31");
+  if (!offsets) return fail(LB_E_ARG, "lb_moe_route: offsets is required");
+  if (T && (!logits || !weights || !experts || !rows || !slots)) return fail(LB_E_ARG, "lb_moe_route: NULL pointer");
+  if (!aligned(logits, dtype == LB_DT_F32 ? 4 : 2) || !aligned(weights, 4) || !aligned(experts, 4) || !aligned(offsets, 4) ||
+      !aligned(rows, 4) || !aligned(slots, 4) || !aligned(workspace, 4))
+    return fail(LB_E_ALIGN, "lb_moe_route: pointers must be element aligned");
+  const int64_t chunks = (T + moe::TOK - 1) / moe::TOK;
+  const size_t need = static_cast<size_t>(chunks) * E * sizeof(int);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(LB_E_WORKSPACE, "lb_moe_route: workspace of %zu bytes needed (got %zu)", need, workspace ? ws_bytes : 0);
+  DevInfo* d;
+  int r = current(&d);
+  if (r) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) return launched(cudaMemsetAsync(offsets, 0, (E + 1) * sizeof(int), st), "moe_route");
+  moe::RouteParams p{logits, dtype, ldl, T, static_cast<int>(E), k, normalize ? 1 : 0, weights, experts, offsets, rows, slots,
+                     static_cast<int*>(workspace)};
+  const unsigned g = static_cast<unsigned>(chunks);
+  const size_t sm = E * sizeof(int);
+  if (E <= 32) moe::route_choose_kernel<1><<<g, 256, sm, st>>>(p);
+  else if (E <= 64) moe::route_choose_kernel<2><<<g, 256, sm, st>>>(p);
+  else if (E <= 128) moe::route_choose_kernel<4><<<g, 256, sm, st>>>(p);
+  else if (E <= 256) moe::route_choose_kernel<8><<<g, 256, sm, st>>>(p);
+  else moe::route_choose_kernel<32><<<g, 256, sm, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return launched(e, "moe_route");
+  moe::route_place_kernel<<<g, 256, 2 * sm, st>>>(p);
+  return launched(cudaGetLastError(), "moe_route");
+}
+
+int lb_moe_combine(const void* z, int64_t rows, int64_t ldz, const float* weights, const int* slots, int64_t T, int k,
+                   int64_t H, int accumulate, void* y, int64_t ldy, void* stream) {
+  if (T < 0 || H <= 0 || k <= 0 || rows < 0 || ldz < H || ldy < H) return fail(LB_E_ARG, "lb_moe_combine: bad sizes");
+  if (T * k > 0x7FFFFFFF || rows > 0x7FFFFFFF) return fail(LB_E_ARG, "lb_moe_combine: T k and rows must be below 2^31");
+  if (T == 0) return LB_OK;
+  if ((!z && rows) || !weights || !slots || !y) return fail(LB_E_ARG, "lb_moe_combine: NULL pointer");
+  if (!aligned(z, 2) || !aligned(y, 2) || !aligned(weights, 4) || !aligned(slots, 4))
+    return fail(LB_E_ALIGN, "lb_moe_combine: pointers must be element aligned");
+  DevInfo* d;
+  int r = current(&d);
+  if (r) return r;
+  int64_t blocks = (T * H + 255) / 256;
+  if (blocks > static_cast<int64_t>(d->sms) * 16) blocks = static_cast<int64_t>(d->sms) * 16;
+  moe::combine_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(z), ldz, rows, weights, slots, T, k, H, static_cast<uint16_t*>(y), ldy, accumulate ? 1 : 0);
+  return launched(cudaGetLastError(), "moe_combine");
+}
+
+}  // extern "C"

@@ -1,0 +1,97 @@
+"""Expert layers on the microscaled products: the router, the way back, and an expert MLP made of them.
+
+    r = route(logits, k)                            # which experts, their weights, the rows in expert order
+    q = microscale.quantize(x, "mxfp4", rows=r.rows, offsets=r.offsets)
+    z = microscale.linear_grouped(q, w)             # each group of rows times its expert's weight
+    y = combine(z, r.weights, r.slots)              # back in token order
+
+``ExpertMLP`` runs that with SwiGLU experts.  The reference's decoders have dense MLPs only (the gate / up / down
+projections of apsi/hub_models.py:1066-1084); the layer here takes the place of one.
+"""
+import ctypes
+from collections import namedtuple
+
+import torch
+
+from . import kernels, microscale
+from ._lib import LB_E_ARG, LB_E_DEVICE, LowbitError, MX_MAX_GROUPS
+from .microscale import _DT, _fn, _launch
+
+__all__ = ["Route", "route", "combine", "ExpertMLP"]
+
+Route = namedtuple("Route", "weights experts offsets rows slots")
+Route.__doc__ = """What ``route`` gives for T tokens over E experts: ``weights`` float32 [T, k]; ``experts`` int32 [T, k], best
+first; ``offsets`` int32 [E + 1], where each expert's rows begin; ``rows`` int32 [T k], the token of each row; ``slots``
+int32 [T, k], the row of each (token, choice)."""
+
+
+def route(logits, k, normalize=True):
+    """The ``k`` experts with the largest logits of each token ([T, E] float32, bfloat16 or float16; equal ones: the lower
+    index), weighted by their softmax over all experts (``normalize``: divided by its sum over the chosen ones), and the
+    T k pairs (token, choice) sorted by expert, in order within one.  A NaN counts as -inf; -inf weighs 0."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise LowbitError(LB_E_DEVICE, "logits must be a CUDA tensor (the B200 path has no CPU fallback)")
+    dt = _DT.get(logits.dtype)
+    if dt is None or logits.dim() != 2:
+        raise LowbitError(LB_E_ARG, f"logits must be float [T, E], got {logits.dtype} {list(logits.shape)}")
+    (T, E), dev = logits.shape, logits.device
+    if not 0 < E <= MX_MAX_GROUPS or not 0 < k <= min(E, 32):
+        raise LowbitError(LB_E_ARG, f"1 to {MX_MAX_GROUPS} experts and k of 1 to min(E, 32), got E = {E}, k = {k}")
+    if E > 1 and logits.stride(1) != 1:
+        raise LowbitError(LB_E_ARG, "the logits of a token must be next to each other")
+    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
+    experts, slots = torch.empty((2, T, k), dtype=torch.int32, device=dev).unbind(0)
+    offsets = torch.empty((E + 1,), dtype=torch.int32, device=dev)
+    rows = torch.empty((T * k,), dtype=torch.int32, device=dev)
+    need = ctypes.c_size_t(0)
+    _fn("lb_moe_route_workspace_size")(T, E, ctypes.byref(need))
+    ws = torch.empty((need.value,), dtype=torch.uint8, device=dev) if need.value else None
+    _launch(dev, "lb_moe_route", logits.data_ptr(), dt, T, E, logits.stride(0) if T > 1 else E, k, 1 if normalize else 0,
+            weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
+            ws.data_ptr() if ws is not None else None, need.value)
+    return Route(weights, experts, offsets, rows, slots)
+
+
+def combine(z, weights, slots, out=None, accumulate=False):
+    """y[t] = sum_j weights[t, j] z[slots[t, j]] (+ out if accumulate) in float32, bfloat16 [T, H].  ``z`` bfloat16
+    [R, H], ``weights`` float32 and ``slots`` int32 [T, k].  A weight of 0 adds nothing, whatever z holds there."""
+    if not isinstance(z, torch.Tensor) or not z.is_cuda:
+        raise LowbitError(LB_E_DEVICE, "z must be a CUDA tensor (the B200 path has no CPU fallback)")
+    dev = z.device
+    if z.dtype != torch.bfloat16 or z.dim() != 2 or (z.shape[1] > 1 and z.stride(1) != 1):
+        raise LowbitError(LB_E_ARG, "z must be bfloat16 [R, H] with unit column stride")
+    for t, dtype, name in ((weights, torch.float32, "weights"), (slots, torch.int32, "slots")):
+        if (not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype or t.dim() != 2 or not t.is_contiguous()
+                or t.shape != weights.shape or t.shape[1] == 0):
+            raise LowbitError(LB_E_ARG, f"{name} must be a contiguous {dtype} tensor [T, k] on {dev}")
+    (T, k), (R, H) = weights.shape, z.shape
+    y, ld = microscale._output(out, T, H, dev, accumulate)
+    _launch(dev, "lb_moe_combine", z.data_ptr(), R, z.stride(0) if R > 1 else H, weights.data_ptr(), slots.data_ptr(), T, k, H,
+            1 if accumulate else 0, y.data_ptr(), ld)
+    return y
+
+
+class ExpertMLP:
+    """A layer of E SwiGLU experts, ``k`` of them for each token, every product in one microscaled format.
+
+    ``router`` [E, H] (any float), ``gate_up`` [E, 2 I, H] with the gate's rows first and ``down`` [E, H, I]: float
+    tensors on the device, quantised here, or ``MxTensor`` (``microscale.pack``).  ``tensor_scales``: the nvfp4 scales of the
+    layer's input and of the hidden activations; found per call where None."""
+
+    def __init__(self, router, gate_up, down, k, fmt="mxfp4", normalize=True, tensor_scales=(None, None)):
+        self.router = router.to(torch.bfloat16).contiguous()
+        self.gate_up, self.down = (w if isinstance(w, microscale.MxTensor) else microscale.quantize(w, fmt)
+                                   for w in (gate_up, down))
+        E, self.H = self.router.shape
+        self.I, self.k, self.fmt, self.normalize, self.tensor_scales = self.down.shape[-1], k, fmt, normalize, tensor_scales
+        if (self.gate_up.shape != (E, 2 * self.I, self.H) or self.down.shape != (E, self.H, self.I)
+                or self.gate_up.fmt != fmt or self.down.fmt != fmt):
+            raise LowbitError(LB_E_ARG, f"router {list(self.router.shape)}, gate_up {self.gate_up} and down {self.down} do not fit")
+
+    def __call__(self, x, out=None, accumulate=False):
+        """x bfloat16 [T, H] -> [T, H] (added to ``out`` if accumulate: the residual)."""
+        r = route(torch.matmul(x, self.router.t()), self.k, self.normalize)
+        q = microscale.quantize(x, self.fmt, self.tensor_scales[0], rows=r.rows, offsets=r.offsets)
+        h = kernels.act_mul(microscale.linear_grouped(q, self.gate_up), self.I, 0) if len(r.rows) else x.new_empty((0, self.I))
+        q = microscale.quantize(h, self.fmt, self.tensor_scales[1], offsets=r.offsets)
+        return combine(microscale.linear_grouped(q, self.down), r.weights, r.slots, out=out, accumulate=accumulate)

@@ -56,6 +56,8 @@ extern "C" {
 #define LB_FMT_FP6_E3M2 7
 #define LB_FMT_FP6_E2M3 8
 #define LB_FMT_FP4_E2M1 9
+#define LB_FMT_MXFP4 10 /* microscaled: e2m1 codes with a scale per block (lb_mx_*); no reference counterpart */
+#define LB_FMT_NVFP4 11
 
 /* element types of weight inputs / dequantised outputs */
 #define LB_DT_F32 0
@@ -68,6 +70,7 @@ extern "C" {
 /* device error word bits (lb_device_errors) */
 #define LB_DEVERR_WAIT_TIMEOUT 1 /* a bounded device-side wait (mbarrier) gave up; the output is invalid */
 #define LB_DEVERR_PEER_TIMEOUT 2 /* lb_rank_barrier gave up waiting for another rank; its output is incomplete */
+#define LB_DEVERR_BAD_INDEX 4    /* a row index or a group offset on the device lay outside its tensor; it was not followed */
 
 /* ---------------------------------------------------------------------------------------------- runtime */
 
@@ -261,6 +264,75 @@ int lb_weight_destroy(lb_weight* w);
  * cudaDeviceReset counts as new): make that call outside stream capture.  No counterpart in the reference. */
 int lb_linear_noalloc(int fmt, const void* x, int64_t M, int64_t K, const void* codes, const void* scales,
                       int64_t N, const void* bias, int accumulate, void* y, int64_t ldy, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- microscaled 4 bits */
+
+/* Rows of 4-bit floats (e2m1 codes) with one scale per block along K.  LB_FMT_MXFP4: blocks of 32, scale 2^(byte - 127);
+ * LB_FMT_NVFP4: blocks of 16, e4m3 scales and one float32 scale t for the tensor.  Any K: a row of codes holds
+ * lb_mx_row_bytes(K) bytes (K rounded up to 32; even element in the low nibble; zeros past K).  The scale bytes lie in
+ * atoms of 512 bytes, 128 rows x 4 block columns, byte (r % 32) 16 + (r / 32 % 4) 4 + c % 4; the atoms of 128 rows
+ * follow each other along the columns, padded with zeros to whole 256 values; lb_mx_scales converts from and to
+ * row-major bytes.  A tensor may consist of groups of rows, each of which begins on 128 rows of scales of its own:
+ * G groups of `per` rows (R = G per; expert weights), or with per == 0 ragged ones, rows [offsets[e], offsets[e + 1])
+ * (device int32 [G + 1], non-decreasing, within [0, R]; others are held in that range and set LB_DEVERR_BAD_INDEX);
+ * G == 0: one group.  G is at most LB_MX_MAX_GROUPS.  The reference has no microscaled format and no experts. */
+#define LB_MX_MAX_GROUPS 1024
+/* Floats behind the first of lb_mx_quant's auto_scale buffer. */
+#define LB_MX_PARTIALS 1023
+
+int64_t lb_mx_row_bytes(int64_t K);
+/* Bytes of the scales of R rows (-1: bad sizes or format). */
+int64_t lb_mx_scale_bytes(int fmt, int64_t R, int64_t K, int64_t G, int64_t per);
+
+/* Quantise R rows: row r is x[rows[r], :] (device int32 indices into the Rin rows of x; one outside gives zeros and sets
+ * LB_DEVERR_BAD_INDEX) or, with rows == NULL, x[r, :].  x: LB_DT_F32, LB_DT_BF16 or LB_DT_F16 with row stride ldx elements.
+ * mxfp4: E = clamp(floor(log2 max|x|) - 2, -127, 127), codes e2m1(x / 2^E).  nvfp4: x' = x / t, s = e4m3(max|x'| / 6), codes
+ * e2m1(x' / s); t = *tensor_scale (device, positive), or with tensor_scale == NULL the smallest power of two with
+ * max|x| / t <= 448 * 6 over all finite values of x, found in a pass of its own and written to auto_scale[0] (device,
+ * 1 + LB_MX_PARTIALS floats).  Nearest, ties to the even code, saturating; a block with a NaN or an infinity gets a
+ * NaN scale.  Rows of no group are not written.  codes and scales 16-byte aligned. */
+int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int64_t ldx, const int* rows, int64_t R,
+                const int* offsets, int64_t G, int64_t per, const float* tensor_scale, float* auto_scale, uint8_t* codes,
+                uint8_t* scales, void* stream);
+
+/* out[r, c] = code * scale (* tensor_scale; NULL: 1), exact in float32 up to the last factor, rounded once to out_dtype. */
+int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, int64_t R, int64_t K,
+                  const int* offsets, int64_t G, int64_t per, void* out, int out_dtype, int64_t ldo, void* stream);
+
+/* Row-major scale bytes [G * N, ld] (one per block of a row) into the layout above (to_atoms != 0), or back. */
+int lb_mx_scales(int fmt, uint8_t* plain, int64_t ld, int64_t G, int64_t N, int64_t K, uint8_t* scales, int to_atoms,
+                 void* stream);
+
+/* y[m, n] = x_t w_t sum_k x[m, k] w[n, k] over the values the codes stand for (+ bias[n], bf16) (+ y[m, n] if accumulate),
+ * float32 accumulation, bf16 out with row stride ldy.  x [M, K] and w [N, K] in the same format, each one group. */
+int lb_mx_linear(int fmt, const uint8_t* x_codes, const uint8_t* x_scales, const float* x_tscale, int64_t M, int64_t K,
+                 const uint8_t* w_codes, const uint8_t* w_scales, const float* w_tscale, int64_t N, const void* bias,
+                 int accumulate, void* y, int64_t ldy, void* stream);
+
+/* The same with a weight of its own for every group of rows: rows [offsets[e], offsets[e + 1]) of x (quantised with those
+ * offsets) times w[e] ([G, N, K], groups of N rows), bias [G, N].  Empty groups cost nothing; rows of no group are not
+ * written. */
+int lb_mx_linear_grouped(int fmt, const uint8_t* x_codes, const uint8_t* x_scales, const float* x_tscale, int64_t M,
+                         int64_t K, const int* offsets, int64_t G, const uint8_t* w_codes, const uint8_t* w_scales,
+                         const float* w_tscale, int64_t N, const void* bias, int accumulate, void* y, int64_t ldy,
+                         void* stream);
+
+/* ---------------------------------------------------------------------------------------------- experts */
+
+/* Routing of T tokens over E experts (1 .. LB_MX_MAX_GROUPS): logits [T, E] (LB_DT_F32 / BF16 / F16, row stride ldl); the k
+ * (1 .. min(E, 32)) largest of each row in falling order, equal ones by index; weights [T, k] = their softmax over all
+ * experts, divided by its sum over the chosen ones if normalize.  NaN counts as -inf, -inf weighs 0, a row of
+ * nothing else weighs 0 throughout, +inf shares the weight evenly.  The T k pairs (t, j) sorted by expert, in order
+ * within one: offsets [E + 1], rows [T k] (the token of each place), slots [T, k] (the place of each pair).  Workspace:
+ * lb_moe_route_workspace_size bytes. */
+int lb_moe_route_workspace_size(int64_t T, int64_t E, size_t* bytes);
+int lb_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, int k, int normalize, float* weights,
+                 int* experts, int* offsets, int* rows, int* slots, void* workspace, size_t ws_bytes, void* stream);
+
+/* y[t, :] (+)= sum_j weights[t, j] z[slots[t, j], :], float32, j in order; bf16 z [rows, H] and y [T, H].  A weight of 0 adds
+ * nothing, whatever z holds there; a slot outside z adds nothing and sets LB_DEVERR_BAD_INDEX. */
+int lb_moe_combine(const void* z, int64_t rows, int64_t ldz, const float* weights, const int* slots, int64_t T, int k,
+                   int64_t H, int accumulate, void* y, int64_t ldy, void* stream);
 
 /* ---------------------------------------------------------------------------------------------- multi-GPU */
 
