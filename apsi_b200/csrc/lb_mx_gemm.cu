@@ -1,6 +1,26 @@
 // Products of microscaled 4-bit operands:  y[m, n] = tx tw sum_b sx[m, b] sw[n, b] sum_{k in b} qx[m, k] qw[n, k]
 // (+ bias[n]) (+ y[m, n]), dense or with one weight per group of rows (experts).
+//
+// The tensor cores multiply the codes and the block scales as they are stored (tcgen05.mma, kind mxf4 / mxf4nvf4 with
+// block_scale), 64 values of K an instruction, float32 accumulators in tensor memory; nothing is expanded.
+// A stage is 256 values of K: 128 bytes of codes a row (one 128-byte swizzled TMA row) of the two operand tiles and their
+// scale atoms, which one 32 x 128-bit copy each puts into tensor memory, a slot per stage, so a slot is not
+// written again before the products that read it are done (the stage's own `empty` barrier).
+//
+//   SWAP = false   few tokens: A = 128 weight rows, B = BT (64 or 128) tokens; an output column is a token, a lane a weight row
+//   SWAP = true    many: A = 128 tokens, B = BT (128 or 256) weight rows; a lane is a token and holds runs of columns
+//
+// Roles (12 warps): 0 TMA, 1 MMA, 4..11 epilogue (warp w reads lanes 32 (w % 4) .. + 31 and half the columns).  BT = 256
+// leaves tensor memory for one accumulator only (256 columns + 4 stages of scales): the epilogue takes it into
+// registers as bf16 at once and stores while the next tile's products run.
+//
+// Few units (decode, small layers): a cluster of S CTAs splits K; each leaves its float32 tile in its own shared
+// memory and every CTA adds its share of the columns over the cluster in rank order: one launch, no workspace, the
+// same bits every time.
+//
+// All mbarrier waits are bounded (lb::mbar_wait); a timeout sets the device error word and the CTA drains.
 #include "lb_mx.cuh"
+#include "lb_tmap.h"
 #include "lb_kernels.h"
 
 namespace lb {
@@ -18,62 +38,473 @@ struct GemmMxParams {
   int64_t M, N, K, ldy;
   int acc;
   Groups g;                 // of the rows of x (ragged); G == 0: dense
+  int ksteps, tiles_w, tiles_t, vec;
 };
 
-// One warp per output, lanes along K.
+constexpr int THREADS = 384;
+constexpr int A_BYTES = 128 * 128;
+constexpr int SMEM_MAX = 227 * 1024;
+
+template <int FMT, int BT>
+struct Cfg {
+  static constexpr int AT = atoms256(FMT);                       // scale atoms of a row block per stage
+  static constexpr int NB = BT > 128 ? 2 : 1;                    // row blocks of the B tile
+  static constexpr int SFA = AT * 512, SFB = NB * AT * 512;
+  static constexpr int STAGE = A_BYTES + BT * 128 + SFA + SFB;
+  static constexpr int STAGES = BT == 256 ? 4 : (BT == 128 ? 6 : (FMT == LB_FMT_MXFP4 ? 8 : 7));
+  static constexpr int ACCS = BT == 256 ? 1 : 2;
+  static constexpr int SF_COLS = AT * 4 * (1 + NB);              // tensor memory columns of a stage's scales
+  static_assert(ACCS * BT + STAGES * SF_COLS <= 512, "tensor memory");
+  static constexpr int PITCH = 129;                              // floats of a column in the cluster's tile
+  static_assert(STAGES * STAGE >= BT * PITCH * 4, "the cluster's tile reuses the stages");
+  static int smem(int G) { return 1024 + STAGES * STAGE + 256 + (G ? (BT == 64 ? 3 : 2) * (G + 1) * 4 : 0); }
+};
+
+__device__ __forceinline__ uint64_t desc_plain(uint32_t addr) {   // 8-row x 16-byte pieces 128 bytes apart, no swizzle
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void tc_cp_scales(uint32_t tmem, uint32_t smem) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc_plain(smem)) : "memory");
+}
 template <int FMT>
-__global__ void __launch_bounds__(256) simple_kernel(const GemmMxParams p) {
-  extern __shared__ int sm[];
-  int* off = sm;
-  int* base = sm + p.g.G + 1;
-  if (p.g.G) load_groups(p.g, p.M, off, base);
-  const int lane = threadIdx.x & 31;
-  const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K), wblocks = (p.N + 127) / 128;
-  const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
-  for (int64_t o = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); o < p.M * p.N;
-       o += static_cast<int64_t>(gridDim.x) * 8) {
-    const int64_t m = o / p.N, n = o - m * p.N;
-    int64_t e = 0, mg = m, xb = 0;
-    if (p.g.G) {
-      e = group_of(off, p.g.G, m);
-      if (e < 0) continue;
-      mg = m - off[e];
-      xb = base[e];
+__device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                          uint32_t accumulate) {
+  if (FMT == LB_FMT_MXFP4)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor: e2m1 operands (K-major), M = 128, N, the scales' type and their first byte in a column
+template <int FMT>
+__device__ __forceinline__ uint32_t idesc_mx(int N, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+         ((FMT == LB_FMT_MXFP4 ? 1u : 0u) << 23) | (8u << 24) | (sf << 29);
+}
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+               : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+
+// One output tile: where its operands and results lie.
+struct Tile {
+  int64_t tok0, wrow;       // first row of x, first row of w's codes
+  int64_t tblk, wblk;       // their row blocks of scales
+  int toff;                 // rows of the first block that lie before tok0 (BT = 64)
+  int tn, nn;               // tokens and weight rows that exist
+  int64_t n0;               // first output column
+  int64_t e;
+};
+
+template <int BT, bool SWAP>
+__device__ __forceinline__ int total_units(const GemmMxParams& p, const int* tiles) {
+  return (p.g.G ? tiles[p.g.G] : p.tiles_t) * p.tiles_w;
+}
+
+// off, base: load_groups; tiles: token tiles before group e (BT = 64; else base itself)
+template <int BT, bool SWAP>
+__device__ __forceinline__ Tile tile_at(const GemmMxParams& p, int u, const int* off, const int* base, const int* tiles) {
+  constexpr int TT = SWAP ? 128 : BT, WT = SWAP ? BT : 128;
+  int t, w, e = 0;
+  int64_t r0 = 0, rows = p.M, blk0 = 0;
+  if (p.g.G) {
+    const int q = u / p.tiles_w;
+    e = group_of(tiles, p.g.G, q);
+    const int te = tiles[e + 1] - tiles[e], v = u - tiles[e] * p.tiles_w;
+    t = v % te;
+    w = v / te;
+    r0 = off[e];
+    rows = off[e + 1] - off[e];
+    blk0 = base[e];
+  } else {                                  // bands of 16 token tiles: a band's weights are read while they are in L2
+    const int band = u / (16 * p.tiles_w), b0 = band * 16;
+    const int bt = p.tiles_t - b0 < 16 ? p.tiles_t - b0 : 16, v = u - b0 * p.tiles_w;
+    t = b0 + v % bt;
+    w = v / bt;
+  }
+  Tile r;
+  r.e = e;
+  r.tok0 = r0 + static_cast<int64_t>(t) * TT;
+  const int64_t left = rows - static_cast<int64_t>(t) * TT;
+  r.tn = static_cast<int>(left < TT ? left : TT);
+  r.tblk = blk0 + (static_cast<int64_t>(t) * TT >> 7);
+  r.toff = (t * TT) & 127;
+  r.n0 = static_cast<int64_t>(w) * WT;
+  r.nn = static_cast<int>(p.N - r.n0 < WT ? p.N - r.n0 : WT);
+  r.wrow = static_cast<int64_t>(e) * p.N + r.n0;
+  r.wblk = static_cast<int64_t>(e) * ((p.N + 127) >> 7) + (r.n0 >> 7);
+  return r;
+}
+
+__device__ __forceinline__ float bias_at(const GemmMxParams& p, int64_t i) {
+  return p.bias ? __uint_as_float(static_cast<uint32_t>(__ldg(p.bias + i)) << 16) : 0.f;
+}
+__device__ __forceinline__ void store_one(const GemmMxParams& p, int64_t m, int64_t n, float v) {
+  uint16_t* yp = p.y + m * p.ldy + n;
+  if (p.acc) v += __uint_as_float(static_cast<uint32_t>(*yp) << 16);
+  *yp = f32_to_bf16_bits_g(v);
+}
+
+constexpr int TOK_BOX = 16;                 // token rows of a TMA box (SWAP = false): only boxes with tokens are read
+
+template <int FMT, int BT, bool SWAP>
+__global__ void __launch_bounds__(THREADS, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const GemmMxParams p) {
+  using C = Cfg<FMT, BT>;
+  constexpr int STAGES = C::STAGES, AT = C::AT;
+  extern __shared__ __align__(1024) uint8_t dyn_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* as = smem;                                            // STAGES x 16 KB
+  uint8_t* bs = as + STAGES * A_BYTES;                           // STAGES x BT x 128
+  uint8_t* sfa = bs + STAGES * BT * 128;
+  uint8_t* sfb = sfa + STAGES * C::SFA;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sfb + STAGES * C::SFB);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;                           // [ACCS]
+  uint64_t* acc_empty = acc_full + 2;                            // [ACCS]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
+  int* off = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + 256);
+  int* base = off + p.g.G + 1;
+  int* tiles = BT == 64 ? base + p.g.G + 1 : base;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    const uint8_t* xr = p.xc + m * rb;
-    const uint8_t* wr = p.wc + (e * p.N + n) * rb;
-    const uint8_t* xsb = p.xs + xb * acols * 512;
-    const uint8_t* wsb = p.ws + e * wblocks * acols * 512;
-    float s = 0.f;
-    for (int64_t w = lane; w < rb / 4; w += 32) {
-      uint32_t a[4], b[4];
-      deq_fp4_word(*reinterpret_cast<const uint32_t*>(xr + 4 * w), a);
-      deq_fp4_word(*reinterpret_cast<const uint32_t*>(wr + 4 * w), b);
-      float d = 0.f;
+    for (int b = 0; b < C::ACCS; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  if (p.g.G) {
+    load_groups(p.g, p.M, off, base);
+    if (BT == 64 && threadIdx.x < 32) {                          // token tiles of 64 before each group
+      int run = 0;
+      for (int e0 = 0; e0 <= p.g.G; e0 += 32) {
+        const int e = e0 + lane;
+        const int n = e < p.g.G ? (off[e + 1] - off[e] + 63) >> 6 : 0;
+        int s = n;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b[i]));
-        d = fmaf(u.x, v.x, fmaf(u.y, v.y, d));
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += v;
+        }
+        if (e <= p.g.G) tiles[e] = run + s - n;
+        run += __shfl_sync(0xffffffffu, s, 31);
       }
-      const int64_t c = w * 8 / block_of(FMT);
-      s = fmaf(scale_value<FMT>(xsb[scale_at(mg, c, acols)]) * scale_value<FMT>(wsb[scale_at(n, c, acols)]), d, s);
     }
-    s = rms_butterfly(s);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  volatile int* abort_v = abort_flag;
+
+  const int S = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+  const int units = total_units<BT, SWAP>(p, tiles);
+  const int u0 = blockIdx.x / S, du = S > 1 ? 0x40000000 : gridDim.x;   // a cluster takes one unit
+  const int kper = (p.ksteps + S - 1) / S;
+  const int k0 = rank * kper, k1 = k0 + kper < p.ksteps ? k0 + kper : p.ksteps;   // may be empty for the last ranks
+  const int64_t acols = static_cast<int64_t>(p.ksteps) * AT;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      float v = s * alpha;
-      if (p.bias) v += __uint_as_float(static_cast<uint32_t>(p.bias[e * p.N + n]) << 16);
-      uint16_t* yp = p.y + m * p.ldy + n;
-      if (p.acc) v += __uint_as_float(static_cast<uint32_t>(*yp) << 16);
-      *yp = f32_to_bf16_bits_g(v);
+      uint32_t it = 0;
+      for (int u = u0; u < units; u += du) {
+        const Tile t = tile_at<BT, SWAP>(p, u, off, base, tiles);
+        const int64_t arow = SWAP ? t.tok0 : t.wrow, brow = SWAP ? t.wrow : t.tok0;
+        const uint8_t* sa = (SWAP ? p.xs + t.tblk * acols * 512 : p.ws + t.wblk * acols * 512);
+        const uint8_t* sb = (SWAP ? p.ws + t.wblk * acols * 512 : p.xs + t.tblk * acols * 512);
+        const int boxes = SWAP ? 1 : (t.tn + TOK_BOX - 1) / TOK_BOX;
+        const int nb = SWAP && BT > 128 ? (t.nn + 127) >> 7 : 1;          // row blocks of B's scales that exist
+        const uint32_t bytes = A_BYTES + (SWAP ? BT : boxes * TOK_BOX) * 128 + C::SFA + nb * C::SFA;
+        for (int ks = k0; ks < k1; ++ks, ++it) {
+          const uint32_t slot = it % STAGES;
+          if (it >= STAGES) mbar_wait(&empty[slot], ((it / STAGES) - 1) & 1, abort_v);
+          mbar_arrive_expect_tx(&full[slot], bytes);
+          tma_load_2d(as + slot * A_BYTES, &tm_a, ks * 128, static_cast<int>(arow), &full[slot]);
+          for (int i = 0; i < boxes; ++i)
+            tma_load_2d(bs + slot * (BT * 128) + i * TOK_BOX * 128, &tm_b, ks * 128, static_cast<int>(brow) + i * TOK_BOX,
+                        &full[slot]);
+          bulk_g2s(sfa + slot * C::SFA, sa + static_cast<int64_t>(ks) * C::SFA, C::SFA, &full[slot]);
+          for (int i = 0; i < nb; ++i)
+            bulk_g2s(sfb + slot * C::SFB + i * C::SFA, sb + (i * acols * 512 + static_cast<int64_t>(ks) * C::SFA), C::SFA,
+                     &full[slot]);
+        }
+      }
     }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      uint32_t it = 0, tc = 0;
+      for (int u = u0; u < units; u += du, ++tc) {
+        const Tile t = tile_at<BT, SWAP>(p, u, off, base, tiles);
+        const int N = SWAP ? BT : (t.tn + 15) / 16 * 16;
+        const uint32_t b = tc % C::ACCS;
+        if (tc >= C::ACCS) mbar_wait(&acc_empty[b], ((tc / C::ACCS) - 1) & 1, abort_v);
+        tc_fence_after();
+        const uint32_t d = tmem + b * BT;
+        for (int ks = k0; ks < k1; ++ks, ++it) {
+          const uint32_t slot = it % STAGES;
+          mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
+          tc_fence_after();
+          const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
+          const uint32_t fa = smem_u32(sfa + slot * C::SFA), fb = smem_u32(sfb + slot * C::SFB);
+#pragma unroll
+          for (int a = 0; a < AT; ++a) {                         // columns [K atom][row block][4]
+            tc_cp_scales(ca + a * 4, fa + a * 512);
+#pragma unroll
+            for (int i = 0; i < C::NB; ++i) tc_cp_scales(cb + a * (4 * C::NB) + i * 4, fb + i * C::SFA + a * 512);
+          }
+          const uint32_t aa = smem_u32(as + slot * A_BYTES), ab = smem_u32(bs + slot * (BT * 128));
+          const int64_t kleft = (p.K + 31) / 32 * 32 - static_cast<int64_t>(ks) * 256;
+          const int nk = kleft >= 256 ? 4 : static_cast<int>((kleft + 63) >> 6);
+          for (int kk = 0; kk < nk; ++kk) {
+            const int a = FMT == LB_FMT_MXFP4 ? kk >> 1 : kk;
+            const uint32_t sf = FMT == LB_FMT_MXFP4 ? (kk & 1) * 2 : 0;
+            tc_mma_mx<FMT>(d, smem_desc_sw128(aa + kk * 32), smem_desc_sw128(ab + kk * 32), idesc_mx<FMT>(N, sf), ca + a * 4,
+                           cb + a * (4 * C::NB) + (SWAP ? 0 : t.toff >> 5), (ks > k0 || kk > 0) ? 1u : 0u);
+          }
+          tc_commit(&empty[slot]);
+        }
+        tc_commit(&acc_full[b]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3, h = (warp - 4) >> 2;                 // lane quarter, half of the columns
+    const int rloc = q * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+    const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
+    constexpr int HALF = BT / 2;
+    uint32_t tc = 0;
+    for (int u = u0; u < units; u += du, ++tc) {
+      const Tile t = tile_at<BT, SWAP>(p, u, off, base, tiles);
+      const uint32_t b = tc % C::ACCS;
+      mbar_wait(&acc_full[b], (tc / C::ACCS) & 1, abort_v);
+      tc_fence_after();
+      const uint32_t d = tmem + lane_addr + b * BT + h * HALF;
+      const int cols = SWAP ? t.nn : t.tn;                       // columns that exist
+      if (S > 1) {                                               // this rank's float32 tile, for the cluster's sum
+        float* part = reinterpret_cast<float*>(smem);
+        for (int c0 = 0; c0 < HALF && h * HALF + c0 < cols; c0 += 16) {
+          uint32_t v[16];
+          tmem_ld_x16(d + c0, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            part[(h * HALF + c0 + j) * C::PITCH + rloc] = k1 > k0 ? __uint_as_float(v[j]) : 0.f;
+        }
+      } else if (!SWAP) {
+        const int64_t n = t.n0 + rloc;
+        const bool ok = rloc < t.nn;
+        const float bias = ok ? bias_at(p, t.e * p.N + n) : 0.f;
+        for (int c0 = 0; c0 < HALF && h * HALF + c0 < cols; c0 += 16) {
+          uint32_t v[16];
+          tmem_ld_x16(d + c0, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int c = h * HALF + c0 + j;
+            if (ok && c < cols) store_one(p, t.tok0 + c, n, __uint_as_float(v[j]) * alpha + bias);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[b]);
+      } else {
+        const int64_t m = t.tok0 + rloc;
+        const bool ok = rloc < t.tn;
+        uint32_t o[HALF / 2];                                    // this row's half as bf16 pairs
+        const int64_t nb0 = t.n0 + h * HALF;
+        uint16_t* yr = p.y + m * p.ldy + nb0;
+#pragma unroll
+        for (int c0 = 0; c0 < HALF; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld_x32(d + c0, v);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float x0 = __uint_as_float(v[2 * j]) * alpha, x1 = __uint_as_float(v[2 * j + 1]) * alpha;
+            const int c = h * HALF + c0 + 2 * j;
+            if (p.bias) {
+              if (c < cols) x0 += bias_at(p, t.e * p.N + t.n0 + c);
+              if (c + 1 < cols) x1 += bias_at(p, t.e * p.N + t.n0 + c + 1);
+            }
+            if (p.acc && ok) {
+              if (c < cols) x0 += __uint_as_float(static_cast<uint32_t>(yr[c0 + 2 * j]) << 16);
+              if (c + 1 < cols) x1 += __uint_as_float(static_cast<uint32_t>(yr[c0 + 2 * j + 1]) << 16);
+            }
+            const __nv_bfloat162 bb = __floats2bfloat162_rn(x0, x1);
+            o[c0 / 2 + j] = *reinterpret_cast<const uint32_t*>(&bb);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[b]);               // the accumulator is free; the stores run on
+        if (ok) {
+#pragma unroll
+          for (int c0 = 0; c0 < HALF; c0 += 8) {
+            const int c = h * HALF + c0;
+            if (p.vec && c + 8 <= cols) {
+              *reinterpret_cast<uint4*>(yr + c0) = make_uint4(o[c0 / 2], o[c0 / 2 + 1], o[c0 / 2 + 2], o[c0 / 2 + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (c + j < cols) yr[c0 + j] = static_cast<uint16_t>(o[(c0 + j) / 2] >> (16 * (j & 1)));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  if (S > 1) {
+    // every CTA adds its share of the columns over the cluster, in rank order
+    __syncwarp();
+    cluster_sync_all();
+    if (u0 < units) {
+      const Tile t = tile_at<BT, SWAP>(p, u0, off, base, tiles);
+      const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
+      const int cols = SWAP ? t.nn : t.tn, lanes = SWAP ? t.tn : t.nn;
+      const int per = (cols + S - 1) / S, c0 = rank * per, c1 = c0 + per < cols ? c0 + per : cols;
+      const int w = c1 - c0;
+      for (int i = threadIdx.x; i < w * 128; i += THREADS) {
+        // consecutive threads take consecutive outputs of a row of y
+        const int c = c0 + (SWAP ? i % w : i >> 7), r = SWAP ? i / w : i & 127;
+        if (r >= lanes) continue;
+        const uint32_t a = smem_u32(smem) + (c * C::PITCH + r) * 4;
+        float v = ld_cluster_f32(a, 0);
+        for (int j = 1; j < S; ++j) v += ld_cluster_f32(a, j);
+        const int64_t m = t.tok0 + (SWAP ? r : c), n = t.n0 + (SWAP ? c : r);
+        store_one(p, m, n, v * alpha + bias_at(p, t.e * p.N + n));
+      }
+    }
+    cluster_sync_all();                     // no CTA leaves while its tile may be read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
-static int launch_product(const char* who, int fmt, const GemmMxParams& p, cudaStream_t st) {
+// ------------------------------------------------------------------------------------------- host side
+static bool encode_codes(CUtensorMap* tm, const uint8_t* codes, int64_t rows, int64_t rb, int box_rows) {
+  PFN_encodeTiled enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(rb), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(rb)};
+  cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t es[2] = {1, 1};
+  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, int BT, bool SWAP>
+static int launch_t(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
+  constexpr int TT = SWAP ? 128 : BT, WT = SWAP ? BT : 128;
+  using C = Cfg<FMT, BT>;
+  const int64_t rb = row_bytes(p.K);
+  p.ksteps = static_cast<int>((p.K + 255) / 256);
+  p.tiles_w = static_cast<int>((p.N + WT - 1) / WT);
+  p.tiles_t = static_cast<int>((p.M + TT - 1) / TT);
+  // the most units there can be: every group may end in a partly filled tile
+  const int64_t tiles = p.g.G ? p.M / TT + (p.g.G < p.M ? p.g.G : p.M) : p.tiles_t;
+  const int64_t units = tiles * p.tiles_w;
+  if (units > 0x3FFFFFFF) return fail(LB_E_ARG, "%s: too many output tiles", who);
+  // K over a cluster while that still fills idle SMs and leaves a rank at least two stages
+  int S = 1;
+  if (BT <= 128)
+    while (S < 8 && units * S * 2 <= sms && p.ksteps >= 4 * S) S *= 2;
+  CUtensorMap tx, tw;
+  if (!encode_codes(&tx, p.xc, p.M, rb, SWAP ? 128 : TOK_BOX) ||
+      !encode_codes(&tw, p.wc, (p.g.G ? p.g.G : 1) * p.N, rb, WT))
+    return fail(LB_E_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
+  const int smem = C::smem(p.g.G);
+  static_assert(1024 + C::STAGES * C::STAGE + 256 + (BT == 64 ? 3 : 2) * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
+  auto kernel = mx_gemm_kernel<FMT, BT, SWAP>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+  if (e != cudaSuccess) return launched(e, who);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(S > 1 ? units * S : (units < sms ? units : sms)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = S;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const CUtensorMap& ta = SWAP ? tx : tw;
+  const CUtensorMap& tb = SWAP ? tw : tx;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, ta, tb, static_cast<const GemmMxParams&>(p)), who);
+}
+
+template <int FMT>
+static int launch_f(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
+  // tokens per weight: all of them, or what a group has on average
+  const int64_t avg = p.g.G ? (p.M + p.g.G - 1) / p.g.G : p.M;
+  if (avg <= 64) return launch_t<FMT, 64, false>(who, p, sms, st);
+  if (avg <= 128) return launch_t<FMT, 128, false>(who, p, sms, st);
+  // 256 weight rows a tile once that gives every SM one
+  const int64_t tiles = ((p.M + 127) / 128) * ((p.N + 255) / 256);
+  if (tiles >= sms) return launch_t<FMT, 256, true>(who, p, sms, st);
+  return launch_t<FMT, 128, true>(who, p, sms, st);
+}
+
+static int launch_product(const char* who, int fmt, GemmMxParams& p, cudaStream_t st) {
   if (!is_mx(fmt)) return fail(LB_E_ARG, "%s: format %d is not microscaled", who, fmt);
   if (p.M < 0 || p.N <= 0 || p.K <= 0 || p.ldy < p.N) return fail(LB_E_ARG, "%s: bad sizes (ldy >= N)", who);
-  if (p.M > 0x7FFFFFFF || p.N > 0x7FFFFF00 || p.K > 0x7FFFFF00) return fail(LB_E_ARG, "%s: M, N and K must be below 2^31", who);
+  if (p.M > 0x7FFFFF00 || p.N > 0x7FFFFF00 || p.K > 0x7FFFFF00 || (p.g.G ? p.g.G : 1) * p.N > 0x7FFFFF00)
+    return fail(LB_E_ARG, "%s: M, K and the weight rows must be below 2^31", who);
   if (p.M == 0) return LB_OK;
   if (!p.xc || !p.xs || !p.wc || !p.ws || !p.y) return fail(LB_E_ARG, "%s: codes, scales and y are required", who);
   if (!aligned(p.xc, 16) || !aligned(p.xs, 16) || !aligned(p.wc, 16) || !aligned(p.ws, 16))
@@ -83,12 +514,8 @@ static int launch_product(const char* who, int fmt, const GemmMxParams& p, cudaS
   DevInfo* d;
   int r = current(&d);
   if (r) return r;
-  const int64_t nb = (p.M * p.N + 7) / 8;
-  const unsigned blocks = static_cast<unsigned>(nb < d->sms * 8 ? nb : d->sms * 8);
-  const size_t sm = p.g.G ? 2 * (p.g.G + 1) * sizeof(int) : 0;
-  if (fmt == LB_FMT_MXFP4) simple_kernel<LB_FMT_MXFP4><<<blocks, 256, sm, st>>>(p);
-  else simple_kernel<LB_FMT_NVFP4><<<blocks, 256, sm, st>>>(p);
-  return launched(cudaGetLastError(), who);
+  p.vec = aligned(p.y, 16) && p.ldy % 8 == 0;
+  return fmt == LB_FMT_MXFP4 ? launch_f<LB_FMT_MXFP4>(who, p, d->sms, st) : launch_f<LB_FMT_NVFP4>(who, p, d->sms, st);
 }
 
 }  // namespace mx
@@ -102,7 +529,7 @@ int lb_mx_linear(int fmt, const uint8_t* x_codes, const uint8_t* x_scales, const
                  const uint8_t* w_codes, const uint8_t* w_scales, const float* w_tscale, int64_t N, const void* bias,
                  int accumulate, void* y, int64_t ldy, void* stream) {
   mx::GemmMxParams p{x_codes, x_scales, x_tscale, w_codes, w_scales, w_tscale, static_cast<const uint16_t*>(bias),
-                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {nullptr, 0, 0}};
+                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {nullptr, 0, 0}, 0, 0, 0, 0};
   return mx::launch_product("lb_mx_linear", fmt, p, static_cast<cudaStream_t>(stream));
 }
 
@@ -114,7 +541,7 @@ int lb_mx_linear_grouped(int fmt, const uint8_t* x_codes, const uint8_t* x_scale
   int r = mx::check_groups("lb_mx_linear_grouped", offsets, G, 0, M);
   if (r) return r;
   mx::GemmMxParams p{x_codes, x_scales, x_tscale, w_codes, w_scales, w_tscale, static_cast<const uint16_t*>(bias),
-                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {offsets, static_cast<int>(G), 0}};
+                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {offsets, static_cast<int>(G), 0}, 0, 0, 0, 0};
   return mx::launch_product("lb_mx_linear_grouped", fmt, p, static_cast<cudaStream_t>(stream));
 }
 
