@@ -108,7 +108,6 @@ __global__ void __launch_bounds__(256) route_choose_kernel(const RouteParams p) 
 // Places: every block adds up the counts it needs, then one warp ranks its chunk's (token, j) in order.
 __global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p) {
   extern __shared__ int next[];                      // [E] next free place of each expert for this chunk
-  __shared__ int carry;
   const int chunks = gridDim.x;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int before = 0, all = 0;
@@ -140,7 +139,6 @@ __global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p) {
       run += __shfl_sync(0xffffffffu, s, 31);
     }
     if (blockIdx.x == 0 && lane == 0) p.offsets[p.E] = run;
-    carry = 0;
     __syncwarp();
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOK;
     const int64_t left = p.T - t0;

@@ -4,15 +4,20 @@
 // The tensor cores multiply the codes and the block scales as they are stored (tcgen05.mma, kind mxf4 / mxf4nvf4 with
 // block_scale), 64 values of K an instruction, float32 accumulators in tensor memory; nothing is expanded.
 // A stage is 256 values of K: 128 bytes of codes a row (one 128-byte swizzled TMA row) of the two operand tiles and their
-// scale atoms, which one 32 x 128-bit copy each puts into tensor memory, a slot per stage, so a slot is not
-// written again before the products that read it are done (the stage's own `empty` barrier).
+// scale atoms.  Four warps move the atoms into tensor memory (tcgen05.st; the four copies in the lane quarters that the
+// products want are one store of each warp), a slot per stage, so a slot is not written again before the products
+// that read it are done (the stage's own `empty` barrier).  As tcgen05.cp they cost the tensor pipe about 45 cycles
+// an atom: with 12 atoms against 512 cycles of nvfp4 products a stage that was the bound.
 //
 //   SWAP = false   few tokens: A = 128 weight rows, B = BT (64 or 128) tokens; an output column is a token, a lane a weight row
-//   SWAP = true    many: A = 128 tokens, B = BT (128 or 256) weight rows; a lane is a token and holds runs of columns
+//   SWAP = true    many: A = 128 tokens, B = BT weight rows; a lane is a token and holds runs of columns
+//   CG = 2         a pair of CTAs (cta_group::2) on 256 tokens x 256 weight rows: each loads its own 128 tokens and half of
+//                  the weight rows, so a product needs 16 KB of codes from L2 for every 128 x 256 outputs and 64 K, not 24;
+//                  with 1-CTA tiles L2 -> SM traffic (12.5 TB/s measured) was the bound
 //
-// Roles (12 warps): 0 TMA, 1 MMA, 4..11 epilogue (warp w reads lanes 32 (w % 4) .. + 31 and half the columns).  BT = 256
-// leaves tensor memory for one accumulator only (256 columns + 4 stages of scales): the epilogue takes it into
-// registers as bf16 at once and stores while the next tile's products run.
+// Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales, 8.. epilogue (4 or 8 warps; warp w reads lanes
+// 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
+// takes it into registers as bf16 at once and stores while the next tile's products run.
 //
 // Few units (decode, small layers): a cluster of S CTAs splits K; each leaves its float32 tile in its own shared
 // memory and every CTA adds its share of the columns over the cluster in rank order: one launch, no workspace, the
@@ -38,55 +43,105 @@ struct GemmMxParams {
   int64_t M, N, K, ldy;
   int acc;
   Groups g;                 // of the rows of x (ragged); G == 0: dense
-  int ksteps, tiles_w, tiles_t, vec;
+  int ksteps, tiles_w, tiles_t;
+  int vec;                  // VEC_*
 };
+constexpr int VEC_Y16 = 1, VEC_Y32 = 2, VEC_BIAS = 4;   // rows of y 16 / 32-byte aligned, rows of bias 16-byte aligned
 
-constexpr int THREADS = 384;
 constexpr int A_BYTES = 128 * 128;
 constexpr int SMEM_MAX = 227 * 1024;
 
-template <int FMT, int BT>
+template <int FMT, int BT, bool SWAP, int CG>
 struct Cfg {
   static constexpr int AT = atoms256(FMT);                       // scale atoms of a row block per stage
   static constexpr int NB = BT > 128 ? 2 : 1;                    // row blocks of the B tile
   static constexpr int SFA = AT * 512, SFB = NB * AT * 512;
-  static constexpr int STAGE = A_BYTES + BT * 128 + SFA + SFB;
-  static constexpr int STAGES = BT == 256 ? 4 : (BT == 128 ? 6 : (FMT == LB_FMT_MXFP4 ? 8 : 7));
+  static constexpr int B_BYTES = BT / CG * 128;                  // a pair's CTAs hold half of B each
+  static constexpr int STAGE = A_BYTES + B_BYTES + SFA + SFB;
+  static constexpr int STAGES = BT == 256 ? (CG == 2 ? (FMT == LB_FMT_MXFP4 ? 6 : 5) : 4)
+                                          : (BT == 128 ? 6 : (FMT == LB_FMT_MXFP4 ? 8 : 7));
   static constexpr int ACCS = BT == 256 ? 1 : 2;
   static constexpr int SF_COLS = AT * 4 * (1 + NB);              // tensor memory columns of a stage's scales
   static_assert(ACCS * BT + STAGES * SF_COLS <= 512, "tensor memory");
   static constexpr int PITCH = 129;                              // floats of a column in the cluster's tile
-  static_assert(STAGES * STAGE >= BT * PITCH * 4, "the cluster's tile reuses the stages");
-  static int smem(int G) { return 1024 + STAGES * STAGE + 256 + (G ? (BT == 64 ? 3 : 2) * (G + 1) * 4 : 0); }
+  static_assert(CG == 2 || STAGES * STAGE >= BT * PITCH * 4, "the cluster's tile reuses the stages");
+  static constexpr int EW = SWAP ? 8 : 4;                        // epilogue warps
+  static constexpr int THREADS = (8 + EW) * 32;
+  static constexpr int COLS = BT / (EW / 4);                     // columns of an epilogue warp
+  static constexpr int TT = SWAP ? 128 * CG : BT, WT = SWAP ? BT : 128;   // tokens and weight rows of a unit
+  static constexpr int LISTS = TT == 128 ? 2 : 3;                // words per group: off, base, (token tiles)
+  static int smem(int G) { return 1024 + STAGES * STAGE + 256 + (G ? LISTS * (G + 1) * 4 : 0); }
+  static_assert(1024 + STAGES * STAGE + 256 + LISTS * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
 };
 
-__device__ __forceinline__ uint64_t desc_plain(uint32_t addr) {   // 8-row x 16-byte pieces 128 bytes apart, no swizzle
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
-}
-__device__ __forceinline__ void tc_cp_scales(uint32_t tmem, uint32_t smem) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc_plain(smem)) : "memory");
-}
-template <int FMT>
+template <int FMT, int CG>
 __device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                           uint32_t accumulate) {
-  if (FMT == LB_FMT_MXFP4)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
+#define LB_MMA_MX(cg, kind)                                                                                            \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                     \
+               "tcgen05.mma.cta_group::" cg ".kind::" kind " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),          \
+               "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                                           \
+               : "memory")
+  if constexpr (FMT == LB_FMT_MXFP4 && CG == 1) LB_MMA_MX("1", "mxf4.block_scale.scale_vec::2X");
+  if constexpr (FMT == LB_FMT_MXFP4 && CG == 2) LB_MMA_MX("2", "mxf4.block_scale.scale_vec::2X");
+  if constexpr (FMT == LB_FMT_NVFP4 && CG == 1) LB_MMA_MX("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  if constexpr (FMT == LB_FMT_NVFP4 && CG == 2) LB_MMA_MX("2", "mxf4nvf4.block_scale.scale_vec::4X");
+#undef LB_MMA_MX
 }
-// Instruction descriptor: e2m1 operands (K-major), M = 128, N, the scales' type and their first byte in a column
-template <int FMT>
+// Instruction descriptor: e2m1 operands (K-major), M = 128 CG, N, the scales' type and their first byte in a column
+template <int FMT, int CG>
 __device__ __forceinline__ uint32_t idesc_mx(int N, uint32_t sf) {
   return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
-         ((FMT == LB_FMT_MXFP4 ? 1u : 0u) << 23) | (8u << 24) | (sf << 29);
+         ((FMT == LB_FMT_MXFP4 ? 1u : 0u) << 23) | (static_cast<uint32_t>(8 * CG) << 24) | (sf << 29);
+}
+// One lane of the warp, chosen so that the compiler knows it is one: what it issues (TMA, products) then takes its operands
+// from uniform registers directly.  Under a test of the lane number each such instruction took over 100 cycles.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+// one scale atom row (four columns) of this warp's 32 lanes
+__device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint4& v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+// commit that arrives on the barrier at the same offset in both CTAs of a pair
+template <int CG>
+__device__ __forceinline__ void tc_commit_all(uint64_t* bar) {
+  if constexpr (CG == 1) tc_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_u32(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+}
+// Arrival on the first CTA's barrier.  What it announces is complete by then and not the thread's own memory writes:
+// tensor memory (tcgen05.wait and the fence before) and TMA's copies (seen on this CTA's barrier).  So the default
+// scope does: an arrival with release at cluster scope held the warp for about 1700 cycles a stage.
+template <int CG>
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  if constexpr (CG == 1) mbar_arrive(bar);
+  else
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+                 "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_all(uint32_t* dst) {
+  if constexpr (CG == 1) {
+    tmem_alloc(dst, 512);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free_all(uint32_t addr) {
+  if constexpr (CG == 1) tmem_dealloc(addr, 512);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -128,15 +183,13 @@ struct Tile {
   int64_t e;
 };
 
-template <int BT, bool SWAP>
 __device__ __forceinline__ int total_units(const GemmMxParams& p, const int* tiles) {
   return (p.g.G ? tiles[p.g.G] : p.tiles_t) * p.tiles_w;
 }
 
-// off, base: load_groups; tiles: token tiles before group e (BT = 64; else base itself)
-template <int BT, bool SWAP>
+// off, base: load_groups; tiles: token tiles before group e (tiles of 128: base itself)
+template <int TT, int WT>
 __device__ __forceinline__ Tile tile_at(const GemmMxParams& p, int u, const int* off, const int* base, const int* tiles) {
-  constexpr int TT = SWAP ? 128 : BT, WT = SWAP ? BT : 128;
   int t, w, e = 0;
   int64_t r0 = 0, rows = p.M, blk0 = 0;
   if (p.g.G) {
@@ -177,55 +230,77 @@ __device__ __forceinline__ void store_one(const GemmMxParams& p, int64_t m, int6
   *yp = f32_to_bf16_bits_g(v);
 }
 
+// v[j] += row[j] (bf16) for the j < n that exist; vec: the row is 16-byte aligned
+__device__ __forceinline__ void add_row(uint32_t (&v)[32], const uint16_t* row, int n, bool vec) {
+  if (vec && n >= 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(row + 8 * i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[8 * i + 2 * j] = __float_as_uint(__uint_as_float(v[8 * i + 2 * j]) + __uint_as_float(w[j] << 16));
+        v[8 * i + 2 * j + 1] = __float_as_uint(__uint_as_float(v[8 * i + 2 * j + 1]) + __uint_as_float(w[j] & 0xFFFF0000u));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(static_cast<uint32_t>(row[j]) << 16));
+  }
+}
+
 constexpr int TOK_BOX = 16;                 // token rows of a TMA box (SWAP = false): only boxes with tokens are read
 
-template <int FMT, int BT, bool SWAP>
-__global__ void __launch_bounds__(THREADS, 1)
+template <int FMT, int BT, bool SWAP, int CG>
+__global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const GemmMxParams p) {
-  using C = Cfg<FMT, BT>;
+  using C = Cfg<FMT, BT, SWAP, CG>;
+  static_assert(CG == 1 || (SWAP && BT == 256), "pairs take 256 x 256 tiles");
   constexpr int STAGES = C::STAGES, AT = C::AT;
   extern __shared__ __align__(1024) uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* as = smem;                                            // STAGES x 16 KB
-  uint8_t* bs = as + STAGES * A_BYTES;                           // STAGES x BT x 128
-  uint8_t* sfa = bs + STAGES * BT * 128;
+  uint8_t* bs = as + STAGES * A_BYTES;                           // STAGES x B_BYTES
+  uint8_t* sfa = bs + STAGES * C::B_BYTES;
   uint8_t* sfb = sfa + STAGES * C::SFA;
   uint64_t* full = reinterpret_cast<uint64_t*>(sfb + STAGES * C::SFB);
   uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;                           // [ACCS]
+  uint64_t* sf_full = empty + STAGES;                            // a stage's scales are in tensor memory
+  uint64_t* acc_full = sf_full + STAGES;                         // [ACCS]
   uint64_t* acc_empty = acc_full + 2;                            // [ACCS]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
   int* abort_flag = reinterpret_cast<int*>(tmem_holder + 1);
   int* off = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + 256);
   int* base = off + p.g.G + 1;
-  int* tiles = BT == 64 ? base + p.g.G + 1 : base;
+  int* tiles = C::LISTS == 3 ? base + p.g.G + 1 : base;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&sf_full[s], 4 * CG);
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
+      mbar_init(&acc_empty[b], C::EW * CG);
     }
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
   }
-  if (warp == 1) {
-    tmem_alloc(tmem_holder, 512);
-    tmem_relinquish();
-  }
+  if (warp == 1) tmem_alloc_all<CG>(tmem_holder);
+  pdl_wait();                                                    // what earlier kernels wrote is read from here on
   if (p.g.G) {
     load_groups(p.g, p.M, off, base);
-    if (BT == 64 && threadIdx.x < 32) {                          // token tiles of 64 before each group
+    if (C::LISTS == 3 && threadIdx.x < 32) {                     // token tiles before each group
       int run = 0;
       for (int e0 = 0; e0 <= p.g.G; e0 += 32) {
         const int e = e0 + lane;
-        const int n = e < p.g.G ? (off[e + 1] - off[e] + 63) >> 6 : 0;
+        const int n = e < p.g.G ? (off[e + 1] - off[e] + C::TT - 1) / C::TT : 0;
         int s = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -239,38 +314,42 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync_all();                               // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   volatile int* abort_v = abort_flag;
 
-  const int S = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
-  const int units = total_units<BT, SWAP>(p, tiles);
-  const int u0 = blockIdx.x / S, du = S > 1 ? 0x40000000 : gridDim.x;   // a cluster takes one unit
+  const int csize = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+  const int S = CG == 2 ? 1 : csize;
+  const int units = total_units(p, tiles);
+  const int u0 = blockIdx.x / csize, du = S > 1 ? 0x40000000 : gridDim.x / csize;   // a splitting cluster takes one unit
   const int kper = (p.ksteps + S - 1) / S;
-  const int k0 = rank * kper, k1 = k0 + kper < p.ksteps ? k0 + kper : p.ksteps;   // may be empty for the last ranks
+  const int k0 = S > 1 ? rank * kper : 0, k1 = k0 + kper < p.ksteps ? k0 + kper : p.ksteps;   // may be empty for the last ranks
   const int64_t acols = static_cast<int64_t>(p.ksteps) * AT;
+  const int half = CG == 2 ? rank : 0;                           // this CTA's half of a pair's tile
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t it = 0;
       for (int u = u0; u < units; u += du) {
-        const Tile t = tile_at<BT, SWAP>(p, u, off, base, tiles);
-        const int64_t arow = SWAP ? t.tok0 : t.wrow, brow = SWAP ? t.wrow : t.tok0;
-        const uint8_t* sa = (SWAP ? p.xs + t.tblk * acols * 512 : p.ws + t.wblk * acols * 512);
+        const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
+        const int64_t arow = SWAP ? t.tok0 + half * 128 : t.wrow, brow = SWAP ? t.wrow + half * 128 : t.tok0;
+        const uint8_t* sa = (SWAP ? p.xs + (t.tblk + half) * acols * 512 : p.ws + t.wblk * acols * 512);
         const uint8_t* sb = (SWAP ? p.ws + t.wblk * acols * 512 : p.xs + t.tblk * acols * 512);
         const int boxes = SWAP ? 1 : (t.tn + TOK_BOX - 1) / TOK_BOX;
         const int nb = SWAP && BT > 128 ? (t.nn + 127) >> 7 : 1;          // row blocks of B's scales that exist
-        const uint32_t bytes = A_BYTES + (SWAP ? BT : boxes * TOK_BOX) * 128 + C::SFA + nb * C::SFA;
+        const int na = half * 128 < t.tn || !SWAP ? 1 : 0;                // and of A's: a pair's second half may have no tokens
+        const uint32_t bytes = A_BYTES + (SWAP ? C::B_BYTES : boxes * TOK_BOX * 128) + (na + nb) * C::SFA;
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
           if (it >= STAGES) mbar_wait(&empty[slot], ((it / STAGES) - 1) & 1, abort_v);
           mbar_arrive_expect_tx(&full[slot], bytes);
           tma_load_2d(as + slot * A_BYTES, &tm_a, ks * 128, static_cast<int>(arow), &full[slot]);
           for (int i = 0; i < boxes; ++i)
-            tma_load_2d(bs + slot * (BT * 128) + i * TOK_BOX * 128, &tm_b, ks * 128, static_cast<int>(brow) + i * TOK_BOX,
+            tma_load_2d(bs + slot * C::B_BYTES + i * TOK_BOX * 128, &tm_b, ks * 128, static_cast<int>(brow) + i * TOK_BOX,
                         &full[slot]);
-          bulk_g2s(sfa + slot * C::SFA, sa + static_cast<int64_t>(ks) * C::SFA, C::SFA, &full[slot]);
+          if (na) bulk_g2s(sfa + slot * C::SFA, sa + static_cast<int64_t>(ks) * C::SFA, C::SFA, &full[slot]);
           for (int i = 0; i < nb; ++i)
             bulk_g2s(sfb + slot * C::SFB + i * C::SFA, sb + (i * acols * 512 + static_cast<int64_t>(ks) * C::SFA), C::SFA,
                      &full[slot]);
@@ -279,10 +358,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    if (half == 0 && elect_one()) {
       uint32_t it = 0, tc = 0;
       for (int u = u0; u < units; u += du, ++tc) {
-        const Tile t = tile_at<BT, SWAP>(p, u, off, base, tiles);
+        const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
         const int N = SWAP ? BT : (t.tn + 15) / 16 * 16;
         const uint32_t b = tc % C::ACCS;
         if (tc >= C::ACCS) mbar_wait(&acc_empty[b], ((tc / C::ACCS) - 1) & 1, abort_v);
@@ -291,39 +370,61 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
           mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
+          mbar_wait(&sf_full[slot], (it / STAGES) & 1, abort_v);
           tc_fence_after();
           const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
-          const uint32_t fa = smem_u32(sfa + slot * C::SFA), fb = smem_u32(sfb + slot * C::SFB);
-#pragma unroll
-          for (int a = 0; a < AT; ++a) {                         // columns [K atom][row block][4]
-            tc_cp_scales(ca + a * 4, fa + a * 512);
-#pragma unroll
-            for (int i = 0; i < C::NB; ++i) tc_cp_scales(cb + a * (4 * C::NB) + i * 4, fb + i * C::SFA + a * 512);
-          }
-          const uint32_t aa = smem_u32(as + slot * A_BYTES), ab = smem_u32(bs + slot * (BT * 128));
+          const uint32_t aa = smem_u32(as + slot * A_BYTES), ab = smem_u32(bs + slot * C::B_BYTES);
           const int64_t kleft = (p.K + 31) / 32 * 32 - static_cast<int64_t>(ks) * 256;
           const int nk = kleft >= 256 ? 4 : static_cast<int>((kleft + 63) >> 6);
           for (int kk = 0; kk < nk; ++kk) {
             const int a = FMT == LB_FMT_MXFP4 ? kk >> 1 : kk;
             const uint32_t sf = FMT == LB_FMT_MXFP4 ? (kk & 1) * 2 : 0;
-            tc_mma_mx<FMT>(d, smem_desc_sw128(aa + kk * 32), smem_desc_sw128(ab + kk * 32), idesc_mx<FMT>(N, sf), ca + a * 4,
-                           cb + a * (4 * C::NB) + (SWAP ? 0 : t.toff >> 5), (ks > k0 || kk > 0) ? 1u : 0u);
+            tc_mma_mx<FMT, CG>(d, smem_desc_sw128(aa + kk * 32), smem_desc_sw128(ab + kk * 32), idesc_mx<FMT, CG>(N, sf),
+                               ca + a * 4, cb + a * (4 * C::NB) + (SWAP ? 0 : t.toff >> 5), (ks > k0 || kk > 0) ? 1u : 0u);
           }
-          tc_commit(&empty[slot]);
+          tc_commit_all<CG>(&empty[slot]);
         }
-        tc_commit(&acc_full[b]);
+        tc_commit_all<CG>(&acc_full[b]);
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 8) {
+    // ------------------------------------------------------------------ scales into tensor memory
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint32_t it = 0;
+    for (int u = u0; u < units; u += du) {
+      for (int ks = k0; ks < k1; ++ks, ++it) {
+        const uint32_t slot = it % STAGES;
+        mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
+        const uint32_t ca = tmem + lane_addr + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
+        const uint32_t fa = smem_u32(sfa + slot * C::SFA) + lane * 16, fb = smem_u32(sfb + slot * C::SFB) + lane * 16;
+        uint4 v[AT * (1 + C::NB)];
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
+          v[a] = lds_v4(fa + a * 512);
+#pragma unroll
+          for (int i = 0; i < C::NB; ++i) v[AT + a * C::NB + i] = lds_v4(fb + i * C::SFA + a * 512);
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int a = 0; a < AT; ++a) tmem_st_x4(ca + a * 4, v[a]);
+#pragma unroll
+        for (int a = 0; a < AT * C::NB; ++a) tmem_st_x4(cb + a * 4, v[AT + a]);   // columns [K atom][row block][4]
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_first<CG>(&sf_full[slot]);
+      }
+    }
+  } else if (warp >= 8) {
     // ------------------------------------------------------------------ epilogue
-    const int q = warp & 3, h = (warp - 4) >> 2;                 // lane quarter, half of the columns
+    const int q = warp & 3, h = (warp - 8) >> 2;                 // lane quarter, part of the columns
     const int rloc = q * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
-    constexpr int HALF = BT / 2;
+    constexpr int HALF = C::COLS;
     uint32_t tc = 0;
     for (int u = u0; u < units; u += du, ++tc) {
-      const Tile t = tile_at<BT, SWAP>(p, u, off, base, tiles);
+      const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
       const uint32_t b = tc % C::ACCS;
       mbar_wait(&acc_full[b], (tc / C::ACCS) & 1, abort_v);
       tc_fence_after();
@@ -347,55 +448,64 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint32_t v[16];
           tmem_ld_x16(d + c0, v);
           tc_wait_ld();
+          uint16_t* yc = p.y + (t.tok0 + h * HALF + c0) * p.ldy + n;
+          const int cl = ok ? cols - h * HALF - c0 : 0;
+          if (p.acc) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int c = h * HALF + c0 + j;
-            if (ok && c < cols) store_one(p, t.tok0 + c, n, __uint_as_float(v[j]) * alpha + bias);
+            for (int j = 0; j < 16; ++j)
+              if (j < cl)
+                v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha + bias +
+                                       __uint_as_float(static_cast<uint32_t>(yc[j * p.ldy]) << 16));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha + bias);
           }
+#pragma unroll
+          for (int j = 0; j < 16; ++j, yc += p.ldy)
+            if (j < cl) *yc = f32_to_bf16_bits_g(__uint_as_float(v[j]));
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[b]);
       } else {
-        const int64_t m = t.tok0 + rloc;
-        const bool ok = rloc < t.tn;
-        uint32_t o[HALF / 2];                                    // this row's half as bf16 pairs
-        const int64_t nb0 = t.n0 + h * HALF;
-        uint16_t* yr = p.y + m * p.ldy + nb0;
+        const int64_t m = t.tok0 + half * 128 + rloc;
+        const bool ok = half * 128 + rloc < t.tn;
+        uint32_t o[HALF / 2];                                    // this row's part as bf16 pairs
+        const int cl = cols - h * HALF;                          // columns of the part that exist
+        uint16_t* yr = p.y + m * p.ldy + t.n0 + h * HALF;
+        const uint16_t* br = p.bias ? p.bias + t.e * p.N + t.n0 + h * HALF : nullptr;
 #pragma unroll
         for (int c0 = 0; c0 < HALF; c0 += 32) {
           uint32_t v[32];
           tmem_ld_x32(d + c0, v);
           tc_wait_ld();
 #pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+          if (br) add_row(v, br + c0, cl - c0, p.vec & VEC_BIAS);
+          if (p.acc && ok) add_row(v, yr + c0, cl - c0, p.vec & VEC_Y16);
+#pragma unroll
           for (int j = 0; j < 16; ++j) {
-            float x0 = __uint_as_float(v[2 * j]) * alpha, x1 = __uint_as_float(v[2 * j + 1]) * alpha;
-            const int c = h * HALF + c0 + 2 * j;
-            if (p.bias) {
-              if (c < cols) x0 += bias_at(p, t.e * p.N + t.n0 + c);
-              if (c + 1 < cols) x1 += bias_at(p, t.e * p.N + t.n0 + c + 1);
-            }
-            if (p.acc && ok) {
-              if (c < cols) x0 += __uint_as_float(static_cast<uint32_t>(yr[c0 + 2 * j]) << 16);
-              if (c + 1 < cols) x1 += __uint_as_float(static_cast<uint32_t>(yr[c0 + 2 * j + 1]) << 16);
-            }
-            const __nv_bfloat162 bb = __floats2bfloat162_rn(x0, x1);
+            const __nv_bfloat162 bb = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
             o[c0 / 2 + j] = *reinterpret_cast<const uint32_t*>(&bb);
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[b]);               // the accumulator is free; the stores run on
+        if (lane == 0) arrive_first<CG>(&acc_empty[b]);          // the accumulator is free; the stores run on
         if (ok) {
+          if ((p.vec & VEC_Y32) && cl >= HALF) {                 // whole 32-byte sectors
 #pragma unroll
-          for (int c0 = 0; c0 < HALF; c0 += 8) {
-            const int c = h * HALF + c0;
-            if (p.vec && c + 8 <= cols) {
-              *reinterpret_cast<uint4*>(yr + c0) = make_uint4(o[c0 / 2], o[c0 / 2 + 1], o[c0 / 2 + 2], o[c0 / 2 + 3]);
-            } else {
+            for (int i = 0; i < HALF / 16; ++i) stg_v8(yr + 16 * i, o + 8 * i);
+          } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (c + j < cols) yr[c0 + j] = static_cast<uint16_t>(o[(c0 + j) / 2] >> (16 * (j & 1)));
+            for (int c0 = 0; c0 < HALF; c0 += 8) {
+              if ((p.vec & VEC_Y16) && c0 + 8 <= cl) {
+                *reinterpret_cast<uint4*>(yr + c0) = make_uint4(o[c0 / 2], o[c0 / 2 + 1], o[c0 / 2 + 2], o[c0 / 2 + 3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (c0 + j < cl) yr[c0 + j] = static_cast<uint16_t>(o[(c0 + j) / 2] >> (16 * (j & 1)));
+              }
             }
           }
         }
@@ -408,12 +518,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
     cluster_sync_all();
     if (u0 < units) {
-      const Tile t = tile_at<BT, SWAP>(p, u0, off, base, tiles);
+      const Tile t = tile_at<C::TT, C::WT>(p, u0, off, base, tiles);
       const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
       const int cols = SWAP ? t.nn : t.tn, lanes = SWAP ? t.tn : t.nn;
       const int per = (cols + S - 1) / S, c0 = rank * per, c1 = c0 + per < cols ? c0 + per : cols;
       const int w = c1 - c0;
-      for (int i = threadIdx.x; i < w * 128; i += THREADS) {
+      for (int i = threadIdx.x; i < w * 128; i += C::THREADS) {
         // consecutive threads take consecutive outputs of a row of y
         const int c = c0 + (SWAP ? i % w : i >> 7), r = SWAP ? i / w : i & 127;
         if (r >= lanes) continue;
@@ -428,9 +538,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (CG == 2) cluster_sync_all();          // neither CTA leaves while the other may arrive on its barriers
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_free_all<CG>(tmem);
   }
 }
 
@@ -447,42 +558,49 @@ static bool encode_codes(CUtensorMap* tm, const uint8_t* codes, int64_t rows, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int FMT, int BT, bool SWAP>
+template <int FMT, int BT, bool SWAP, int CG>
 static int launch_t(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
-  constexpr int TT = SWAP ? 128 : BT, WT = SWAP ? BT : 128;
-  using C = Cfg<FMT, BT>;
+  using C = Cfg<FMT, BT, SWAP, CG>;
   const int64_t rb = row_bytes(p.K);
   p.ksteps = static_cast<int>((p.K + 255) / 256);
-  p.tiles_w = static_cast<int>((p.N + WT - 1) / WT);
-  p.tiles_t = static_cast<int>((p.M + TT - 1) / TT);
+  p.tiles_w = static_cast<int>((p.N + C::WT - 1) / C::WT);
+  p.tiles_t = static_cast<int>((p.M + C::TT - 1) / C::TT);
   // the most units there can be: every group may end in a partly filled tile
-  const int64_t tiles = p.g.G ? p.M / TT + (p.g.G < p.M ? p.g.G : p.M) : p.tiles_t;
+  const int64_t tiles = p.g.G ? p.M / C::TT + (p.g.G < p.M ? p.g.G : p.M) : p.tiles_t;
   const int64_t units = tiles * p.tiles_w;
-  if (units > 0x3FFFFFFF) return fail(LB_E_ARG, "%s: too many output tiles", who);
+  if (units > 0x3FFFFFFF / 8) return fail(LB_E_ARG, "%s: too many output tiles", who);
   // K over a cluster while that still fills idle SMs and leaves a rank at least two stages
   int S = 1;
   if (BT <= 128)
     while (S < 8 && units * S * 2 <= sms && p.ksteps >= 4 * S) S *= 2;
+  const int cl = CG == 2 ? 2 : S;
   CUtensorMap tx, tw;
   if (!encode_codes(&tx, p.xc, p.M, rb, SWAP ? 128 : TOK_BOX) ||
-      !encode_codes(&tw, p.wc, (p.g.G ? p.g.G : 1) * p.N, rb, WT))
+      !encode_codes(&tw, p.wc, (p.g.G ? p.g.G : 1) * p.N, rb, SWAP ? BT / CG : 128))
     return fail(LB_E_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
-  const int smem = C::smem(p.g.G);
-  static_assert(1024 + C::STAGES * C::STAGE + 256 + (BT == 64 ? 3 : 2) * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
-  auto kernel = mx_gemm_kernel<FMT, BT, SWAP>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
-  if (e != cudaSuccess) return launched(e, who);
+  auto kernel = mx_gemm_kernel<FMT, BT, SWAP, CG>;
+  static std::atomic<uint64_t> ready{0};                          // devices whose limit is set
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+    if (e != cudaSuccess) return launched(e, who);
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(S > 1 ? units * S : (units < sms ? units : sms)));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
+  const int64_t persist = units * cl < sms ? units * cl : sms / cl * cl;
+  cfg.gridDim = dim3(static_cast<unsigned>(S > 1 ? units * S : persist));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::smem(p.g.G);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = S;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cl;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cl > 1 ? 2 : 1;
   const CUtensorMap& ta = SWAP ? tx : tw;
   const CUtensorMap& tb = SWAP ? tw : tx;
   return launched(cudaLaunchKernelEx(&cfg, kernel, ta, tb, static_cast<const GemmMxParams&>(p)), who);
@@ -492,12 +610,12 @@ template <int FMT>
 static int launch_f(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
   // tokens per weight: all of them, or what a group has on average
   const int64_t avg = p.g.G ? (p.M + p.g.G - 1) / p.g.G : p.M;
-  if (avg <= 64) return launch_t<FMT, 64, false>(who, p, sms, st);
-  if (avg <= 128) return launch_t<FMT, 128, false>(who, p, sms, st);
-  // 256 weight rows a tile once that gives every SM one
-  const int64_t tiles = ((p.M + 127) / 128) * ((p.N + 255) / 256);
-  if (tiles >= sms) return launch_t<FMT, 256, true>(who, p, sms, st);
-  return launch_t<FMT, 128, true>(who, p, sms, st);
+  if (avg <= 64) return launch_t<FMT, 64, false, 1>(who, p, sms, st);
+  if (avg <= 128) return launch_t<FMT, 128, false, 1>(who, p, sms, st);
+  // 256 x 256 a pair of SMs once that gives every pair one
+  const int64_t tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (tiles >= sms / 2) return launch_t<FMT, 256, true, 2>(who, p, sms, st);
+  return launch_t<FMT, 128, true, 1>(who, p, sms, st);
 }
 
 static int launch_product(const char* who, int fmt, GemmMxParams& p, cudaStream_t st) {
@@ -514,7 +632,8 @@ static int launch_product(const char* who, int fmt, GemmMxParams& p, cudaStream_
   DevInfo* d;
   int r = current(&d);
   if (r) return r;
-  p.vec = aligned(p.y, 16) && p.ldy % 8 == 0;
+  p.vec = (aligned(p.y, 16) && p.ldy % 8 == 0 ? VEC_Y16 : 0) | (aligned(p.y, 32) && p.ldy % 16 == 0 ? VEC_Y32 : 0) |
+          (aligned(p.bias, 16) && p.N % 8 == 0 ? VEC_BIAS : 0);
   return fmt == LB_FMT_MXFP4 ? launch_f<LB_FMT_MXFP4>(who, p, d->sms, st) : launch_f<LB_FMT_NVFP4>(who, p, d->sms, st);
 }
 
