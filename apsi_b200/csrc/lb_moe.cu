@@ -161,25 +161,88 @@ __global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p) {
   }
 }
 
-__global__ void __launch_bounds__(256) combine_kernel(const uint16_t* __restrict__ z, int64_t ldz, int64_t rows,
-                                                      const float* __restrict__ w, const int* __restrict__ slots,
-                                                      int64_t T, int k, int64_t H, uint16_t* __restrict__ y, int64_t ldy,
-                                                      int acc) {
-  const int64_t total = T * H;
+struct CombineParams {
+  const uint16_t* z;
+  int64_t ldz, rows;
+  const float* w;
+  const int* slots;
+  int64_t T;
+  int k;
+  int64_t H;
+  uint16_t* y;
+  int64_t ldy;
+  int acc;
+};
+
+// One thread per eight columns of a token (VEC) or one: the loads of up to eight rows are in flight together; j in order.
+template <bool VEC>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int C = VEC ? 8 : 1, U = VEC ? 4 : 8;
+  const int64_t hc = VEC ? p.H / 8 : p.H, total = p.T * hc;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = i / H, h = i - t * H;
-    float s = acc ? __uint_as_float(static_cast<uint32_t>(y[t * ldy + h]) << 16) : 0.f;
-    for (int j = 0; j < k; ++j) {
-      const float wj = w[t * k + j];
-      const int r = slots[t * k + j];
-      if (r < 0 || r >= rows) {
-        atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
-        continue;
+    const int64_t t = total <= 0xFFFFFFFFll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(hc) : i / hc;
+    const int64_t h = (i - t * hc) * C;
+    float s[C];
+    uint16_t* yp = p.y + t * p.ldy + h;
+#pragma unroll
+    for (int c = 0; c < C; ++c) s[c] = 0.f;
+    if (p.acc) {
+      if constexpr (VEC) {
+        const uint4 u = *reinterpret_cast<const uint4*>(yp);
+        const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) { s[2 * c] = __uint_as_float(v[c] << 16); s[2 * c + 1] = __uint_as_float(v[c] & 0xFFFF0000u); }
+      } else {
+        s[0] = __uint_as_float(static_cast<uint32_t>(*yp) << 16);
       }
-      if (wj != 0.f) s = fmaf(wj, __uint_as_float(static_cast<uint32_t>(z[r * ldz + h]) << 16), s);
     }
-    y[t * ldy + h] = f32_to_bf16_bits_g(s);
+    for (int j0 = 0; j0 < p.k; j0 += U) {
+      float wj[U];
+      uint4 v[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        wj[j] = 0.f;
+        if (j0 + j < p.k) {
+          const int r = __ldg(p.slots + t * p.k + j0 + j);
+          if (r < 0 || r >= p.rows) {
+            atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
+          } else {
+            wj[j] = __ldg(p.w + t * p.k + j0 + j);
+            const uint16_t* zp = p.z + r * p.ldz + h;
+            if constexpr (VEC) v[j] = ldg_nc_v4(zp);
+            else v[j].x = static_cast<uint32_t>(*zp) << 16;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (wj[j] == 0.f) continue;
+        if constexpr (VEC) {
+          const uint32_t u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            s[2 * c] = fmaf(wj[j], __uint_as_float(u[c] << 16), s[2 * c]);
+            s[2 * c + 1] = fmaf(wj[j], __uint_as_float(u[c] & 0xFFFF0000u), s[2 * c + 1]);
+          }
+        } else {
+          s[0] = fmaf(wj[j], __uint_as_float(v[j].x), s[0]);
+        }
+      }
+    }
+    if constexpr (VEC) {
+      uint32_t o[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(s[2 * c], s[2 * c + 1]);
+        o[c] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *reinterpret_cast<uint4*>(yp) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+      *yp = f32_to_bf16_bits_g(s[0]);
+    }
   }
 }
 
@@ -244,11 +307,15 @@ int lb_moe_combine(const void* z, int64_t rows, int64_t ldz, const float* weight
   DevInfo* d;
   int r = current(&d);
   if (r) return r;
-  int64_t blocks = (T * H + 255) / 256;
+  moe::CombineParams p{static_cast<const uint16_t*>(z), ldz, rows, weights, slots, T, k, H, static_cast<uint16_t*>(y), ldy,
+                       accumulate ? 1 : 0};
+  const bool vec = H % 8 == 0 && ldz % 8 == 0 && ldy % 8 == 0 && aligned(z, 16) && aligned(y, 16);
+  int64_t blocks = (T * (vec ? H / 8 : H) + 255) / 256;
   if (blocks > static_cast<int64_t>(d->sms) * 16) blocks = static_cast<int64_t>(d->sms) * 16;
-  moe::combine_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(z), ldz, rows, weights, slots, T, k, H, static_cast<uint16_t*>(y), ldy, accumulate ? 1 : 0);
-  return launched(cudaGetLastError(), "moe_combine");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return launched(vec ? mx::launch_early(moe::combine_kernel<true>, static_cast<int>(blocks), 0, st, p)
+                      : mx::launch_early(moe::combine_kernel<false>, static_cast<int>(blocks), 0, st, p),
+                  "moe_combine");
 }
 
 }  // extern "C"

@@ -34,33 +34,35 @@ struct In<LB_DT_F16> {
   static __device__ __forceinline__ float one(const void* p, int64_t i) { return __half2float(static_cast<const __half*>(p)[i]); }
 };
 
-// 16 values of a row from column c0 (zeros past K); vec: rows are 16-byte aligned
+// 16 values of a row from column c0 (zeros past K); vec: rows are aligned to 32 bytes (2), 16 (1) or their elements (0)
 template <int DT>
-__device__ __forceinline__ void load16(const void* row, int64_t c0, int64_t K, bool vec, float (&v)[16]) {
+__device__ __forceinline__ void load16(const void* row, int64_t c0, int64_t K, int vec, float (&v)[16]) {
   if (vec && c0 + 16 <= K) {
     const char* p = static_cast<const char*>(row) + c0 * In<DT>::SIZE;
+    uint32_t w[DT == LB_DT_F32 ? 16 : 8];
+#pragma unroll
+    for (int i = 0; i < In<DT>::SIZE / 2; ++i) {
+      if (vec == 2) {
+        ldg_nc_v8(p + 32 * i, *reinterpret_cast<uint32_t(*)[8]>(&w[8 * i]));
+      } else {
+        const uint4 a = ldg_nc_v4(p + 32 * i), b = ldg_nc_v4(p + 32 * i + 16);
+        w[8 * i] = a.x; w[8 * i + 1] = a.y; w[8 * i + 2] = a.z; w[8 * i + 3] = a.w;
+        w[8 * i + 4] = b.x; w[8 * i + 5] = b.y; w[8 * i + 6] = b.z; w[8 * i + 7] = b.w;
+      }
+    }
     if constexpr (DT == LB_DT_F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 u = ldg_nc_v4(p + 16 * i);
-        v[4 * i] = __uint_as_float(u.x); v[4 * i + 1] = __uint_as_float(u.y);
-        v[4 * i + 2] = __uint_as_float(u.z); v[4 * i + 3] = __uint_as_float(u.w);
-      }
+      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 u = ldg_nc_v4(p + 16 * i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (DT == LB_DT_BF16) {
-            v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-            v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-          } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            v[8 * i + 2 * j] = f.x;
-            v[8 * i + 2 * j + 1] = f.y;
-          }
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (DT == LB_DT_BF16) {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
         }
       }
     }
@@ -68,6 +70,34 @@ __device__ __forceinline__ void load16(const void* row, int64_t c0, int64_t K, b
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = c0 + i < K ? In<DT>::one(row, c0 + i) : 0.f;
   }
+}
+
+// Codes of y / s without 16 divisions.  y of a 16-bit type scaled by a power of two has at most 11 significant bits and
+// s 4, so a quotient that is no tie is at least 2^-11 away from every tie, relatively: y times the rounded inverse is
+// within 2^-22 of it, and rounding that to 16 significant bits puts every tie back on its place and moves nothing across one.
+__device__ __forceinline__ void codes_short(const float (&y)[16], float rs, uint32_t& lo, uint32_t& hi) {
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float((__float_as_uint(y[i] * rs) + 0x80u) & 0xFFFFFF00u);
+  lo = e2m1_codes(v);
+  hi = e2m1_codes(v + 8);
+}
+// For any y: the codes of slightly more and slightly less than y / s (2^-20 either way, past the rounding of the inverse and
+// the product).  The quotient's code lies between; where the two differ (about one group of eight in 10^5 of random values)
+// the eight quotients are divided out.
+__device__ __forceinline__ uint32_t codes8_any(const float* y, float s, float rs) {
+  float up[8], dn[8];
+  const float ru = rs * (1.f + 0x1p-20f), rd = rs * (1.f - 0x1p-20f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    up[i] = y[i] * ru;
+    dn[i] = y[i] * rd;
+  }
+  const uint32_t a = e2m1_codes(up);
+  if (a == e2m1_codes(dn)) return a;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) up[i] = __fdiv_rn(y[i], s);
+  return e2m1_codes(up);
 }
 
 struct QuantParams {
@@ -94,17 +124,38 @@ __device__ __forceinline__ float auto_scale(float amax) {
   return pow2f(e < -126 ? -126 : e);
 }
 
-// One thread per 16 values, a warp per 512 values of one row.
+// Where row r lies: its place in its group and the group's first row block (false: it is in no group).
+__device__ __forceinline__ bool place_of(const Groups& g, const int* off, const int* base, int64_t gblocks, int64_t r,
+                                         int64_t& rg, int64_t& blk0) {
+  rg = r;
+  blk0 = 0;
+  if (g.G == 0) return true;
+  int64_t e;
+  if (g.per > 0) {
+    e = static_cast<uint32_t>(r) / static_cast<uint32_t>(g.per);
+    rg = r - e * g.per;
+    blk0 = e * gblocks;
+  } else {
+    e = group_of(off, g.G, r);
+    if (e < 0) return false;
+    rg = r - off[e];
+    blk0 = base[e];
+  }
+  return true;
+}
+
+// One thread per 16 values, a warp per 512 values of one row.  Memory-bound: 32-byte loads, whole sectors; the next row's
+// index is on its way while this row is rounded.
 template <int FMT, int DT>
 __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
   extern __shared__ int sm[];
   pdl_launch_dependents();
+  pdl_wait();
   int* off = sm;
   int* base = sm + p.g.G + 1;
   __shared__ float s_t;
   const int lane = threadIdx.x & 31;
-  const bool ragged = p.g.G > 0 && p.g.per == 0;
-  if (ragged) load_groups(p.g, p.R, off, base);
+  if (p.g.G > 0 && p.g.per == 0) load_groups(p.g, p.R, off, base);
   if (FMT == LB_FMT_NVFP4) {
     if (p.part) {
       if (threadIdx.x < 32) {
@@ -127,45 +178,39 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
   const bool pow2 = FMT == LB_FMT_NVFP4 && (__float_as_uint(t) & 0x807FFFFFu) == 0 && t >= pow2f(-126) && t <= pow2f(126);
   const float inv = 1.0f / t;
   const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K);
-  const int64_t segs = (p.K + 511) / 512;
-  const int64_t nseg = p.R * segs;
+  const uint32_t segs = static_cast<uint32_t>((p.K + 511) / 512);
+  const int64_t nseg = p.R * segs, step = static_cast<int64_t>(gridDim.x) * 8;
   const int64_t gblocks = p.g.per > 0 ? (p.g.per + 127) / 128 : 0;
-  for (int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < nseg;
-       w += static_cast<int64_t>(gridDim.x) * 8) {
-    const int64_t r = w / segs;
-    const int64_t c0 = (w - r * segs) * 512 + lane * 16;
-    int64_t rg = r, blk0 = 0;                  // row in its group, the group's first row block
-    if (ragged) {
-      const int e = group_of(off, p.g.G, r);
-      if (e < 0) continue;                     // rows of no group are left alone
-      rg = r - off[e];
-      blk0 = base[e];
-    } else if (p.g.per > 0) {
-      const int64_t e = r / p.g.per;
-      rg = r - e * p.g.per;
-      blk0 = e * gblocks;
-    }
-    int64_t src = r;
-    if (p.rows) {
-      src = p.rows[r];
-      if (src < 0 || src >= p.Rin) {           // no such row: zeros, and the error word says so
-        if (lane == 0) atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
-        src = -1;
-      }
-    }
+  auto split = [&](int64_t w, int64_t& r, int64_t& c) {          // warp item -> row, first column
+    r = nseg <= 0xFFFFFFFFll ? static_cast<uint32_t>(w) / segs : w / segs;
+    c = (w - r * segs) * 512;
+  };
+  int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), r, c0;
+  split(w < nseg ? w : 0, r, c0);
+  int64_t src = p.rows && w < nseg ? p.rows[r] : r;
+  while (w < nseg) {
+    const int64_t wn = w + step;
+    int64_t rn, cn;
+    split(wn < nseg ? wn : 0, rn, cn);
+    c0 += lane * 16;
     float v[16];
-    if (src >= 0) load16<DT>(static_cast<const char*>(p.x) + src * p.ldx * In<DT>::SIZE, c0, p.K, p.vec, v);
-    else {
+    if (src >= 0 && src < p.Rin) {
+      load16<DT>(static_cast<const char*>(p.x) + src * p.ldx * In<DT>::SIZE, c0, p.K, p.vec, v);
+    } else {                                                     // no such row: zeros, and the error word says so
+      if (lane == 0) atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.f;
     }
+    const int64_t srcn = p.rows && wn < nseg ? p.rows[rn] : rn;
+    int64_t rg, blk0;
+    const bool in = place_of(p.g, off, base, gblocks, r, rg, blk0);   // rows of no group are left alone
     uint32_t am = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
       am = b > am ? b : am;
     }
-    uint32_t byte;
+    uint32_t byte, lo, hi;
     if (FMT == LB_FMT_MXFP4) {
       const uint32_t o = __shfl_xor_sync(0xffffffffu, am, 1);
       am = o > am ? o : am;
@@ -174,28 +219,41 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
       const float mul = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= mul;
+      lo = e2m1_codes(v);
+      hi = e2m1_codes(v + 8);
     } else {
       const bool bad = am >= 0x7F800000u;
       float a = __uint_as_float(am);
       a = pow2 ? a * inv : __fdiv_rn(a, t);
       byte = bad ? 0x7Fu : e4m3_byte(__fdiv_rn(a, 6.0f));
-      const float s = e4m3_value(byte);
+      const float s = e4m3_value(byte), rs = byte == 0u || bad ? 0.f : 1.0f / s;   // no scale: zeros with their signs
+      if (pow2) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float y = pow2 ? v[i] * inv : __fdiv_rn(v[i], t);
-        v[i] = byte == 0u || bad ? copysignf(0.f, y) : __fdiv_rn(y, s);
+        for (int i = 0; i < 16; ++i) v[i] *= inv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __fdiv_rn(v[i], t);
+      }
+      if (DT != LB_DT_F32 && pow2) {
+        codes_short(v, rs, lo, hi);
+      } else {
+        lo = codes8_any(v, s, rs);
+        hi = codes8_any(v + 8, s, rs);
       }
     }
-    if (c0 < rb * 2)
-      *reinterpret_cast<uint2*>(p.codes + r * rb + c0 / 2) = make_uint2(e2m1_codes(v), e2m1_codes(v + 8));
+    if (in && c0 < rb * 2) *reinterpret_cast<uint2*>(p.codes + r * rb + c0 / 2) = make_uint2(lo, hi);
     // four scale bytes of neighbouring blocks make one word
     constexpr int PER = FMT == LB_FMT_MXFP4 ? 2 : 1;
     uint32_t word = byte;
     word |= __shfl_down_sync(0xffffffffu, word, PER) << 8;
     word = (word & 0xFFFFu) | (__shfl_down_sync(0xffffffffu, word, 2 * PER) << 16);
     const int64_t c = c0 / block_of(FMT);
-    if (lane % (4 * PER) == 0 && c < acols * 4)
+    if (in && lane % (4 * PER) == 0 && c < acols * 4)
       *reinterpret_cast<uint32_t*>(p.scales + blk0 * acols * 512 + scale_at(rg, c, acols)) = word;
+    w = wn;
+    r = rn;
+    c0 = cn;
+    src = srcn;
   }
 }
 
@@ -205,6 +263,7 @@ __global__ void __launch_bounds__(256) amax_kernel(const void* __restrict__ x, i
                                                    float* __restrict__ part) {
   __shared__ uint32_t red[8];
   pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t segs = (K + 511) / 512, nseg = R * segs;
   uint32_t am = 0;
@@ -236,38 +295,30 @@ struct DequantParams {
   int64_t R, K, ldo;
   Groups g;
   void* out;
-  int out_dt, vec;
+  int vec;                  // as load16's
 };
 
 // One thread per 16 values.
-template <int FMT>
+template <int FMT, int ODT>
 __global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) {
   extern __shared__ int sm[];
+  pdl_launch_dependents();
+  pdl_wait();
   int* off = sm;
   int* base = sm + p.g.G + 1;
-  const bool ragged = p.g.G > 0 && p.g.per == 0;
-  if (ragged) load_groups(p.g, p.R, off, base);
+  if (p.g.G > 0 && p.g.per == 0) load_groups(p.g, p.R, off, base);
   const float t = FMT == LB_FMT_NVFP4 && p.t ? *p.t : 1.f;
   const int lane = threadIdx.x & 31;
   const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K);
-  const int64_t segs = (p.K + 511) / 512, nseg = p.R * segs;
+  const uint32_t segs = static_cast<uint32_t>((p.K + 511) / 512);
+  const int64_t nseg = p.R * segs;
   const int64_t gblocks = p.g.per > 0 ? (p.g.per + 127) / 128 : 0;
   for (int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < nseg;
        w += static_cast<int64_t>(gridDim.x) * 8) {
-    const int64_t r = w / segs;
+    const int64_t r = nseg <= 0xFFFFFFFFll ? static_cast<uint32_t>(w) / segs : w / segs;
     const int64_t c0 = (w - r * segs) * 512 + lane * 16;
-    int64_t rg = r, blk0 = 0;
-    if (ragged) {
-      const int e = group_of(off, p.g.G, r);
-      if (e < 0) continue;
-      rg = r - off[e];
-      blk0 = base[e];
-    } else if (p.g.per > 0) {
-      const int64_t e = r / p.g.per;
-      rg = r - e * p.g.per;
-      blk0 = e * gblocks;
-    }
-    if (c0 >= p.K) continue;
+    int64_t rg, blk0;
+    if (c0 >= p.K || !place_of(p.g, off, base, gblocks, r, rg, blk0)) continue;
     const uint2 q = *reinterpret_cast<const uint2*>(p.codes + r * rb + c0 / 2);
     const float s = scale_value<FMT>(p.scales[blk0 * acols * 512 + scale_at(rg, c0 / block_of(FMT), acols)]);
     uint32_t h[8];
@@ -289,20 +340,15 @@ __global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) 
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= t;
     }
-    if (p.out_dt == LB_DT_F32) {
-      float* o = static_cast<float*>(p.out) + r * p.ldo + c0;
-      if (p.vec && c0 + 16 <= p.K) {
+    constexpr int NW = ODT == LB_DT_F32 ? 16 : 8, ES = ODT == LB_DT_F32 ? 4 : 2;
+    uint32_t u[NW];
+    if constexpr (ODT == LB_DT_F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) if (c0 + i < p.K) o[i] = v[i];
-      }
+      for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i]);
     } else {
-      uint32_t u[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (p.out_dt == LB_DT_BF16) {
+        if constexpr (ODT == LB_DT_BF16) {
           const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
           u[i] = *reinterpret_cast<const uint32_t*>(&b);
         } else {
@@ -310,13 +356,24 @@ __global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) 
           u[i] = *reinterpret_cast<const uint32_t*>(&b);
         }
       }
-      uint16_t* o = static_cast<uint16_t*>(p.out) + r * p.ldo + c0;
-      if (p.vec && c0 + 16 <= p.K) {
-        reinterpret_cast<uint4*>(o)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-        reinterpret_cast<uint4*>(o)[1] = make_uint4(u[4], u[5], u[6], u[7]);
-      } else {
+    }
+    char* o = static_cast<char*>(p.out) + (r * p.ldo + c0) * ES;
+    if (p.vec && c0 + 16 <= p.K) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) if (c0 + i < p.K) o[i] = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
+      for (int i = 0; i < NW / 8; ++i) {
+        if (p.vec == 2) {
+          stg_v8(o + 32 * i, u + 8 * i);
+        } else {
+          reinterpret_cast<uint4*>(o)[2 * i] = make_uint4(u[8 * i], u[8 * i + 1], u[8 * i + 2], u[8 * i + 3]);
+          reinterpret_cast<uint4*>(o)[2 * i + 1] = make_uint4(u[8 * i + 4], u[8 * i + 5], u[8 * i + 6], u[8 * i + 7]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (c0 + i >= p.K) continue;
+        if constexpr (ODT == LB_DT_F32) reinterpret_cast<uint32_t*>(o)[i] = u[i];
+        else reinterpret_cast<uint16_t*>(o)[i] = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
       }
     }
   }
@@ -347,6 +404,25 @@ constexpr int MAX_PARTS = LB_MX_PARTIALS;
 static int quant_blocks(int64_t R, int64_t K, int sms) {
   const int64_t nseg = R * ((K + 511) / 512), b = (nseg + 7) / 8;
   return static_cast<int>(b < static_cast<int64_t>(sms) * 8 ? b : static_cast<int64_t>(sms) * 8);
+}
+// 2: rows are 32-byte aligned, 1: 16, 0: neither
+static int row_vec(const void* p, int64_t ld, int es) {
+  return aligned(p, 32) && ld * es % 32 == 0 ? 2 : (aligned(p, 16) && ld * es % 16 == 0 ? 1 : 0);
+}
+// A launch that may begin while the kernel before it ends (it waits for that one before it touches memory).
+template <typename P>
+static cudaError_t launch_early(void (*kernel)(P), int blocks, size_t smem, cudaStream_t st, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 static bool is_mx(int fmt) { return fmt == LB_FMT_MXFP4 || fmt == LB_FMT_NVFP4; }
 static int dt_size(int dt) { return dt == LB_DT_F32 ? 4 : 2; }
@@ -407,7 +483,7 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
   p.t = tensor_scale;
   p.part = nullptr; p.t_out = nullptr; p.nparts = 0;
   p.codes = codes; p.scales = scales;
-  p.vec = aligned(x, 16) && ldx * es % 16 == 0;
+  p.vec = mx::row_vec(x, ldx, es);
   if (fmt == LB_FMT_NVFP4 && !tensor_scale) {
     int nb = mx::quant_blocks(Rin, K, d->sms);
     if (nb > mx::MAX_PARTS) nb = mx::MAX_PARTS;
@@ -423,16 +499,15 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
   }
   const int blocks = mx::quant_blocks(R, K, d->sms);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
-#define LB_MX_QUANT(F)                                                                                         \
-  do {                                                                                                         \
-    if (x_dtype == LB_DT_F32) mx::quant_kernel<F, LB_DT_F32><<<blocks, 256, sm, st>>>(p);                      \
-    else if (x_dtype == LB_DT_BF16) mx::quant_kernel<F, LB_DT_BF16><<<blocks, 256, sm, st>>>(p);               \
-    else mx::quant_kernel<F, LB_DT_F16><<<blocks, 256, sm, st>>>(p);                                           \
-  } while (0)
+  cudaError_t e;
+#define LB_MX_QUANT(F)                                                                                              \
+  e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::quant_kernel<F, LB_DT_F32>, blocks, sm, st, p)                 \
+      : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::quant_kernel<F, LB_DT_BF16>, blocks, sm, st, p)                \
+                              : mx::launch_early(mx::quant_kernel<F, LB_DT_F16>, blocks, sm, st, p)
   if (fmt == LB_FMT_MXFP4) LB_MX_QUANT(LB_FMT_MXFP4);
   else LB_MX_QUANT(LB_FMT_NVFP4);
 #undef LB_MX_QUANT
-  return launched(cudaGetLastError(), "mx_quant");
+  return launched(e, "mx_quant");
 }
 
 int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const float* tensor_scale, int64_t R, int64_t K,
@@ -450,14 +525,20 @@ int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const fl
     return fail(LB_E_ALIGN, "lb_mx_dequant: codes and scales must be 16-byte, the others element aligned");
   DevInfo* d;
   if ((r = current(&d))) return r;
-  mx::DequantParams p{codes, scales, tensor_scale, R, K, ldo, {offsets, static_cast<int>(G), per}, out, out_dtype,
-                      aligned(out, 16) && ldo * es % 16 == 0};
+  mx::DequantParams p{codes, scales, tensor_scale, R, K, ldo, {offsets, static_cast<int>(G), per}, out,
+                      mx::row_vec(out, ldo, es)};
   const int blocks = mx::quant_blocks(R, K, d->sms);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (fmt == LB_FMT_MXFP4) mx::dequant_kernel_mx<LB_FMT_MXFP4><<<blocks, 256, sm, st>>>(p);
-  else mx::dequant_kernel_mx<LB_FMT_NVFP4><<<blocks, 256, sm, st>>>(p);
-  return launched(cudaGetLastError(), "mx_dequant");
+  cudaError_t e;
+#define LB_MX_DEQUANT(F)                                                                                            \
+  e = out_dtype == LB_DT_F32    ? mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_F32>, blocks, sm, st, p)           \
+      : out_dtype == LB_DT_BF16 ? mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_BF16>, blocks, sm, st, p)          \
+                                : mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_F16>, blocks, sm, st, p)
+  if (fmt == LB_FMT_MXFP4) LB_MX_DEQUANT(LB_FMT_MXFP4);
+  else LB_MX_DEQUANT(LB_FMT_NVFP4);
+#undef LB_MX_DEQUANT
+  return launched(e, "mx_dequant");
 }
 
 int lb_mx_scales(int fmt, uint8_t* plain, int64_t ld, int64_t G, int64_t N, int64_t K, uint8_t* scales, int to_atoms,

@@ -8,14 +8,13 @@
 ``ExpertMLP`` runs that with SwiGLU experts.  The reference's decoders have dense MLPs only (the gate / up / down
 projections of apsi/hub_models.py:1066-1084); the layer here takes the place of one.
 """
-import ctypes
 from collections import namedtuple
 
 import torch
 
 from . import kernels, microscale
 from ._lib import LB_E_ARG, LB_E_DEVICE, LowbitError, MX_MAX_GROUPS
-from .microscale import _DT, _fn, _launch
+from .microscale import _DT, _launch, _output
 
 __all__ = ["Route", "route", "combine", "ExpertMLP"]
 
@@ -34,22 +33,21 @@ def route(logits, k, normalize=True):
     dt = _DT.get(logits.dtype)
     if dt is None or logits.dim() != 2:
         raise LowbitError(LB_E_ARG, f"logits must be float [T, E], got {logits.dtype} {list(logits.shape)}")
-    (T, E), dev = logits.shape, logits.device
+    T, E = logits.shape
     if not 0 < E <= MX_MAX_GROUPS or not 0 < k <= min(E, 32):
         raise LowbitError(LB_E_ARG, f"1 to {MX_MAX_GROUPS} experts and k of 1 to min(E, 32), got E = {E}, k = {k}")
     if E > 1 and logits.stride(1) != 1:
         raise LowbitError(LB_E_ARG, "the logits of a token must be next to each other")
-    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
-    experts, slots = torch.empty((2, T, k), dtype=torch.int32, device=dev).unbind(0)
-    offsets = torch.empty((E + 1,), dtype=torch.int32, device=dev)
-    rows = torch.empty((T * k,), dtype=torch.int32, device=dev)
-    need = ctypes.c_size_t(0)
-    _fn("lb_moe_route_workspace_size")(T, E, ctypes.byref(need))
-    ws = torch.empty((need.value,), dtype=torch.uint8, device=dev) if need.value else None
-    _launch(dev, "lb_moe_route", logits.data_ptr(), dt, T, E, logits.stride(0) if T > 1 else E, k, 1 if normalize else 0,
-            weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-            ws.data_ptr() if ws is not None else None, need.value)
-    return Route(weights, experts, offsets, rows, slots)
+    n = T * k
+    weights = logits.new_empty((T, k), dtype=torch.float32)
+    # experts, slots, rows, offsets and the workspace (one count per expert and 64 tokens) in one allocation
+    ints = logits.new_empty(3 * n + E + 1 + (T + 63) // 64 * E, dtype=torch.int32)
+    experts, slots, rows, offsets, _ = ints.split((n, n, n, E + 1, ints.shape[0] - 3 * n - E - 1))
+    at = ints.data_ptr()
+    _launch(logits.get_device(), "lb_moe_route", logits.data_ptr(), dt, T, E, logits.stride(0) if T > 1 else E, k,
+            1 if normalize else 0, weights.data_ptr(), at, at + 12 * n, at + 8 * n, at + 4 * n, at + 12 * n + 4 * (E + 1),
+            4 * ((T + 63) // 64 * E))
+    return Route(weights, experts.view(T, k), offsets, rows, slots.view(T, k))
 
 
 def combine(z, weights, slots, out=None, accumulate=False):
@@ -57,15 +55,15 @@ def combine(z, weights, slots, out=None, accumulate=False):
     [R, H], ``weights`` float32 and ``slots`` int32 [T, k].  A weight of 0 adds nothing, whatever z holds there."""
     if not isinstance(z, torch.Tensor) or not z.is_cuda:
         raise LowbitError(LB_E_DEVICE, "z must be a CUDA tensor (the B200 path has no CPU fallback)")
-    dev = z.device
+    dev = z.get_device()
     if z.dtype != torch.bfloat16 or z.dim() != 2 or (z.shape[1] > 1 and z.stride(1) != 1):
         raise LowbitError(LB_E_ARG, "z must be bfloat16 [R, H] with unit column stride")
     for t, dtype, name in ((weights, torch.float32, "weights"), (slots, torch.int32, "slots")):
-        if (not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype or t.dim() != 2 or not t.is_contiguous()
+        if (not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype != dtype or t.dim() != 2 or not t.is_contiguous()
                 or t.shape != weights.shape or t.shape[1] == 0):
-            raise LowbitError(LB_E_ARG, f"{name} must be a contiguous {dtype} tensor [T, k] on {dev}")
+            raise LowbitError(LB_E_ARG, f"{name} must be a contiguous {dtype} tensor [T, k] on {z.device}")
     (T, k), (R, H) = weights.shape, z.shape
-    y, ld = microscale._output(out, T, H, dev, accumulate)
+    y, ld = _output(out, T, H, z, accumulate)
     _launch(dev, "lb_moe_combine", z.data_ptr(), R, z.stride(0) if R > 1 else H, weights.data_ptr(), slots.data_ptr(), T, k, H,
             1 if accumulate else 0, y.data_ptr(), ld)
     return y

@@ -16,7 +16,7 @@ of range is not followed and sets ``DEVERR_BAD_INDEX`` (``kernels.device_errors`
 """
 import torch
 
-from . import _lib
+from . import _lib, kernels
 from ._lib import DT_BF16, DT_F16, DT_F32, LB_E_ARG, LB_E_DEVICE, LowbitError, MICROSCALED_FMT, MX_MAX_GROUPS, MX_PARTIALS
 
 __all__ = ["MxTensor", "quantize", "dequantize", "pack", "plain_scales", "linear", "linear_grouped"]
@@ -40,16 +40,20 @@ def _err(msg):
 def _cuda(t, name):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise LowbitError(LB_E_DEVICE, f"{name} must be a CUDA tensor (the B200 path has no CPU fallback)")
-    return t
+
+
+_cur_dev = kernels._cur_dev or torch.cuda.current_device
+_stream = kernels._raw_stream or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _launch(dev, name, *args):
-    """One call of the library on ``dev``'s current stream (the last argument)."""
-    if dev.index == torch.cuda.current_device():
-        rc = _fn(name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    """One call of the library on the current stream (its last argument) of the device with index ``dev``."""
+    f = _fns.get(name) or _fn(name)
+    if dev == _cur_dev():
+        rc = f(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = _fn(name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = f(*args, _stream(dev))
     if rc:
         _lib.check(rc)
 
@@ -79,19 +83,38 @@ class MxTensor:
     """Microscaled rows: ``fmt``; ``shape`` ([R, K], or [E, N, K] for one matrix per expert); ``codes`` uint8
     [rows, row bytes]; ``scales`` uint8, in the tensor cores' order (``plain_scales`` gives rows); ``tensor_scale``
     float32 [1] (nvfp4; else None); ``offsets`` int32 [G + 1] when the rows are ragged groups (else None)."""
-    __slots__ = ("fmt", "shape", "codes", "scales", "tensor_scale", "offsets")
+    # one buffer holds codes, scales and a tensor scale that was found: one allocation a call; the views are made when asked for
+    __slots__ = ("fmt", "shape", "rows", "offsets", "_buf", "_keep", "_codes", "_scales", "_t", "_dev", "_tail")
 
-    def __init__(self, fmt, shape, codes, scales, tensor_scale=None, offsets=None):
-        self.fmt, self.shape, self.codes, self.scales = fmt, shape, codes, scales
-        self.tensor_scale, self.offsets = tensor_scale, offsets
+    def __init__(self, fmt, shape, rows, buf, codes, scales, t, offsets, keep=None, tail=0):
+        """``codes``, ``scales``, ``t``: addresses (in ``buf``, or in the tensors ``keep``: codes, scales, tensor scale)."""
+        self.fmt, self.shape, self.rows, self.offsets = fmt, shape, rows, offsets
+        self._buf, self._keep, self._codes, self._scales, self._t, self._tail = buf, keep, codes, scales, t, tail
+        self._dev = buf.get_device()
 
     @property
     def device(self):
-        return self.codes.device
+        return self._buf.device
 
     @property
-    def rows(self):
-        return self.shape[0] if len(self.shape) == 2 else self.shape[0] * self.shape[1]
+    def codes(self):
+        if self._keep is not None and self._keep[0] is not None:
+            return self._keep[0]
+        rb = _row_bytes(self.shape[-1])
+        return self._buf[:self.rows * rb].view(self.rows, rb)
+
+    @property
+    def scales(self):
+        if self._keep is not None and self._keep[1] is not None:
+            return self._keep[1]
+        at = self.rows * _row_bytes(self.shape[-1])
+        return self._buf[at:self._buf.numel() - self._tail]
+
+    @property
+    def tensor_scale(self):
+        if self._keep is not None and self._keep[2] is not None:
+            return self._keep[2]
+        return self._buf[-self._tail:][:4].view(torch.float32) if self._tail else None
 
     def _groups(self):
         """(G, per) as the library takes them."""
@@ -100,6 +123,7 @@ class MxTensor:
         return (0, 0) if len(self.shape) == 2 else (self.shape[0], self.shape[1])
 
     def nbytes(self):
+        """Bytes of codes and scales."""
         return self.codes.numel() + self.scales.numel()
 
     def dequantize(self, dtype=torch.float32):
@@ -110,9 +134,10 @@ class MxTensor:
 
 
 def _index(t, name, dev):
-    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-        raise _err(f"{name} must be a contiguous int32 vector on {dev}")
-    return t
+    """The length of a vector of row indices or offsets."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise _err(f"{name} must be a contiguous int32 vector on the operands' device")
+    return t.shape[0]
 
 
 def _tensor_scale(fmt, t, dev):
@@ -121,12 +146,12 @@ def _tensor_scale(fmt, t, dev):
             raise _err(f"{fmt} has no tensor scale")
         return None
     if t is None or isinstance(t, torch.Tensor):
-        if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
-            raise _err(f"tensor_scale must be one float32 value on {dev}")
+        if t is not None and (t.get_device() != dev or t.dtype != torch.float32 or t.numel() != 1):
+            raise _err("tensor_scale must be one float32 value on the operands' device")
         return t
     if not 0.0 < float(t) < float("inf"):
         raise _err(f"tensor_scale must be positive and finite, got {t}")
-    return torch.full((1,), float(t), dtype=torch.float32, device=dev)
+    return torch.full((1,), float(t), dtype=torch.float32, device=torch.device("cuda", dev))
 
 
 def quantize(x, fmt, tensor_scale=None, rows=None, offsets=None):
@@ -141,41 +166,42 @@ def quantize(x, fmt, tensor_scale=None, rows=None, offsets=None):
     dt = _DT.get(x.dtype)
     if dt is None:
         raise _err(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    dev, shape = x.device, tuple(x.shape)
+    dev, shape = x.get_device(), tuple(x.shape)
     G = per = 0
-    if len(shape) == 3:
+    if len(shape) == 2:
+        R_in, K = shape
+        ldx = x.stride(0) if R_in > 1 else max(K, 1)
+    elif len(shape) == 3:
         if not x.is_contiguous() or rows is not None or offsets is not None:
             raise _err("one matrix per expert [E, N, K] must be contiguous, with neither rows nor offsets")
         G, per, K = shape
         if not 0 < G <= MX_MAX_GROUPS:
-            raise _err(f"at most {MX_MAX_GROUPS} experts, got {G}")
+            raise _err(f"1 to {MX_MAX_GROUPS} experts, got {G}")
         R_in, ldx = G * per, K
-    elif len(shape) == 2:
-        R_in, K = shape
-        ldx = x.stride(0) if R_in > 1 else max(K, 1)
     else:
         raise _err(f"x must be [R, K] or [E, N, K], got {list(shape)}")
     if K == 0 or x.stride(-1) != 1 and K > 1:
         raise _err("the values of a row must be next to each other, and at least one")
     R = R_in
     if rows is not None:
-        R = _index(rows, "rows", dev).numel()
+        R = _index(rows, "rows", dev)
         shape = (R, K)
     if offsets is not None:
-        G = _index(offsets, "offsets", dev).numel() - 1
+        G = _index(offsets, "offsets", dev) - 1
         if not 0 < G <= MX_MAX_GROUPS:
             raise _err(f"offsets must hold 2 to {MX_MAX_GROUPS + 1} values, got {G + 1}")
     t = _tensor_scale(fmt, tensor_scale, dev)
-    auto = None
-    if t is None and f == _lib.FMT_NVFP4:
-        auto = torch.empty((1 + MX_PARTIALS,), dtype=torch.float32, device=dev)
-        if R == 0:
-            auto[0] = 1.0
-    codes = torch.empty((R, _row_bytes(K)), dtype=torch.uint8, device=dev)
-    scales = torch.empty((_scale_bytes(fmt, R, K, G, per),), dtype=torch.uint8, device=dev)
-    _launch(dev, "lb_mx_quant", f, x.data_ptr(), dt, R_in, K, ldx, _ptr(rows), R, _ptr(offsets), G, per, _ptr(t), _ptr(auto),
-            codes.data_ptr(), scales.data_ptr())
-    return MxTensor(fmt, shape, codes, scales, t if auto is None else auto[:1], offsets)
+    nc, ns = R * _row_bytes(K), _scale_bytes(fmt, R, K, G, per)
+    tail = 4 * (1 + MX_PARTIALS) if t is None and fmt == "nvfp4" else 0
+    buf = x.new_empty(nc + ns + tail, dtype=torch.uint8)
+    codes = buf.data_ptr()
+    found = codes + nc + ns if tail else None
+    if tail and R == 0:
+        buf[nc + ns:].view(torch.float32)[0] = 1.0
+    _launch(dev, "lb_mx_quant", f, x.data_ptr(), dt, R_in, K, ldx, _ptr(rows), R, _ptr(offsets), G, per, _ptr(t), found, codes,
+            codes + nc)
+    return MxTensor(fmt, shape, R, buf, codes, codes + nc, found if t is None else t.data_ptr(), offsets,
+                    None if t is None else (None, None, t), tail)
 
 
 def dequantize(q, dtype=torch.float32):
@@ -184,10 +210,10 @@ def dequantize(q, dtype=torch.float32):
     if dt is None:
         raise _err(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     G, per = q._groups()
-    K, dev = q.shape[-1], q.codes.device
-    out = torch.empty(q.shape, dtype=dtype, device=dev)
-    _launch(dev, "lb_mx_dequant", MICROSCALED_FMT[q.fmt], q.codes.data_ptr(), q.scales.data_ptr(), _ptr(q.tensor_scale), q.rows, K,
-            _ptr(q.offsets), G, per, out.data_ptr(), dt, K)
+    K = q.shape[-1]
+    out = q._buf.new_empty(q.shape, dtype=dtype)
+    _launch(q._dev, "lb_mx_dequant", MICROSCALED_FMT[q.fmt], q._codes, q._scales, q._t, q.rows, K, _ptr(q.offsets), G, per,
+            out.data_ptr(), dt, K)
     return out
 
 
@@ -196,11 +222,11 @@ def pack(codes, scales, K, fmt, tensor_scale=None):
     [E, N, ...], ``scales`` [N, >= blocks] or [E, N, ...]: uint8, or the float8 type whose bytes they are."""
     f = _format(fmt)
     _cuda(codes, "codes")
-    dev, lead = codes.device, tuple(codes.shape[:-1])
+    dev, lead = codes.get_device(), tuple(codes.shape[:-1])
     if codes.dtype != torch.uint8 or len(lead) not in (1, 2) or 0 in lead:
         raise _err("codes must be uint8 [N, bytes] or [E, N, bytes]")
-    if not isinstance(scales, torch.Tensor) or scales.device != dev or scales.element_size() != 1 or tuple(scales.shape[:-1]) != lead:
-        raise _err(f"scales must be one byte per block, {list(lead)} rows of them, on {dev}")
+    if not isinstance(scales, torch.Tensor) or scales.get_device() != dev or scales.element_size() != 1 or tuple(scales.shape[:-1]) != lead:
+        raise _err(f"scales must be one byte per block, {list(lead)} rows of them, on {codes.device}")
     nb = -(-K // _BLOCK[fmt])
     if K <= 0 or codes.shape[-1] < (K + 1) // 2 or scales.shape[-1] < nb:
         raise _err(f"K = {K} needs {(K + 1) // 2} code bytes and {nb} scales a row")
@@ -210,17 +236,16 @@ def pack(codes, scales, K, fmt, tensor_scale=None):
     rb = _row_bytes(K)
     flat = codes.reshape(G * N, codes.shape[-1])
     if K % 32 or flat.shape[1] != rb or not flat.is_contiguous() or flat.data_ptr() % 16:
-        full = torch.zeros((G * N, rb), dtype=torch.uint8, device=dev)
+        full = codes.new_zeros((G * N, rb))
         full[:, :(K + 1) // 2] = flat[:, :(K + 1) // 2]
         if K % 2:
             full[:, K // 2] &= 15
         flat = full
     s = scales.view(torch.uint8).reshape(G * N, -1)[:, :nb].contiguous()
-    atoms = torch.empty((_scale_bytes(fmt, N * G, K, G if len(lead) == 2 else 0, N if len(lead) == 2 else 0),),
-                        dtype=torch.uint8, device=dev)
+    atoms = codes.new_empty(_scale_bytes(fmt, N * G, K, *((G, N) if len(lead) == 2 else (0, 0))))
     _launch(dev, "lb_mx_scales", f, s.data_ptr(), nb, G, N, K, atoms.data_ptr(), 1)
     t = _tensor_scale(fmt, 1.0 if tensor_scale is None and fmt == "nvfp4" else tensor_scale, dev)
-    return MxTensor(fmt, lead + (K,), flat, atoms, t)
+    return MxTensor(fmt, lead + (K,), G * N, atoms, flat.data_ptr(), atoms.data_ptr(), _ptr(t), None, (flat, atoms, t))
 
 
 def plain_scales(q):
@@ -231,17 +256,18 @@ def plain_scales(q):
     K, nb = q.shape[-1], -(-q.shape[-1] // _BLOCK[q.fmt])
     out = torch.empty((*q.shape[:-1], nb), dtype=torch.uint8, device=q.device)
     if out.numel():
-        _launch(q.device, "lb_mx_scales", MICROSCALED_FMT[q.fmt], out.data_ptr(), nb, G, N, K, q.scales.data_ptr(), 0)
+        _launch(q._dev, "lb_mx_scales", MICROSCALED_FMT[q.fmt], out.data_ptr(), nb, G, N, K, q._scales, 0)
     return out
 
 
-def _output(out, M, N, dev, accumulate):
+def _output(out, M, N, like, accumulate):
+    """(output, its row stride): ``out`` checked, or a new bfloat16 [M, N] on ``like``'s device."""
     if out is None:
         if accumulate:
             raise _err("accumulate needs an output tensor")
-        return torch.empty((M, N), dtype=torch.bfloat16, device=dev), N
-    if not isinstance(out, torch.Tensor) or out.device != dev or out.dtype != torch.bfloat16:
-        raise _err(f"out must be a bfloat16 tensor on {dev}")
+        return like.new_empty((M, N), dtype=torch.bfloat16), N
+    if not isinstance(out, torch.Tensor) or out.get_device() != like.get_device() or out.dtype != torch.bfloat16:
+        raise _err(f"out must be a bfloat16 tensor on {like.device}")
     if out.dim() != 2 or out.shape[0] != M or out.shape[1] != N or (out.stride(1) != 1 and N > 1):
         raise _err(f"out must be [{M}, {N}] with unit column stride")
     ld = out.stride(0) if M > 1 else N
@@ -251,10 +277,12 @@ def _output(out, M, N, dev, accumulate):
 
 
 def _bias(bias, n, dev):
-    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.device != dev or bias.dtype != torch.bfloat16
-                             or bias.numel() != n or not bias.is_contiguous()):
-        raise _err(f"bias must be a contiguous bfloat16 tensor of {n} values on {dev}")
-    return bias
+    if bias is None:
+        return None
+    if (not isinstance(bias, torch.Tensor) or bias.get_device() != dev or bias.dtype != torch.bfloat16 or bias.numel() != n
+            or not bias.is_contiguous()):
+        raise _err(f"bias must be a contiguous bfloat16 tensor of {n} values on the operands' device")
+    return bias.data_ptr()
 
 
 def linear(x, w, bias=None, out=None, accumulate=False, tensor_scale=None):
@@ -268,15 +296,15 @@ def linear(x, w, bias=None, out=None, accumulate=False, tensor_scale=None):
     if not isinstance(x, MxTensor):
         _cuda(x, "x")
         lead = x.shape[:-1]
-        x = quantize(x.reshape(-1, x.shape[-1]), w.fmt, tensor_scale)
-    if x.fmt != w.fmt or len(x.shape) != 2 or x.offsets is not None or x.shape[1] != w.shape[1] or x.device != w.device:
-        raise _err(f"x must be {w.fmt} [M, {w.shape[1]}] in one group on {w.device}, got {x}")
-    (M, K), N, dev = x.shape, w.shape[0], w.codes.device
-    y, ld = _output(out, M, N, dev, accumulate)
-    _launch(dev, "lb_mx_linear", MICROSCALED_FMT[w.fmt], x.codes.data_ptr(), x.scales.data_ptr(), _ptr(x.tensor_scale), M, K,
-            w.codes.data_ptr(), w.scales.data_ptr(), _ptr(w.tensor_scale), N, _ptr(_bias(bias, N, dev)), 1 if accumulate else 0,
-            y.data_ptr(), ld)
-    return y if lead is None or out is not None else y.view(*lead, N)
+        x = quantize(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, w.fmt, tensor_scale)
+    N, K = w.shape
+    if x.fmt != w.fmt or len(x.shape) != 2 or x.offsets is not None or x.shape[1] != K or x._dev != w._dev:
+        raise _err(f"x must be {w.fmt} [M, {K}] in one group on {w.device}, got {x}")
+    M, dev = x.shape[0], w._dev
+    y, ld = _output(out, M, N, w._buf, accumulate)
+    _launch(dev, "lb_mx_linear", MICROSCALED_FMT[w.fmt], x._codes, x._scales, x._t, M, K, w._codes, w._scales, w._t, N,
+            _bias(bias, N, dev), 1 if accumulate else 0, y.data_ptr(), ld)
+    return y if lead is None or len(lead) == 1 or out is not None else y.view(*lead, N)
 
 
 def linear_grouped(x, w, bias=None, out=None, accumulate=False):
@@ -287,12 +315,11 @@ def linear_grouped(x, w, bias=None, out=None, accumulate=False):
     if not isinstance(w, MxTensor) or len(w.shape) != 3:
         raise _err("w must be an MxTensor [E, N, K]")
     E, N, K = w.shape
-    if (not isinstance(x, MxTensor) or x.fmt != w.fmt or x.offsets is None or x.shape[1] != K or x.device != w.device
-            or x.offsets.numel() != E + 1):
+    if (not isinstance(x, MxTensor) or x.fmt != w.fmt or x.offsets is None or x.shape[1] != K or x._dev != w._dev
+            or x.offsets.shape[0] != E + 1):
         raise _err(f"x must be an MxTensor {w.fmt} [R, {K}] on {w.device} quantised with the offsets of {E} groups, got {x}")
-    M, dev = x.shape[0], w.codes.device
-    y, ld = _output(out, M, N, dev, accumulate)
-    _launch(dev, "lb_mx_linear_grouped", MICROSCALED_FMT[w.fmt], x.codes.data_ptr(), x.scales.data_ptr(), _ptr(x.tensor_scale), M, K,
-            x.offsets.data_ptr(), E, w.codes.data_ptr(), w.scales.data_ptr(), _ptr(w.tensor_scale), N, _ptr(_bias(bias, E * N, dev)),
-            1 if accumulate else 0, y.data_ptr(), ld)
+    M, dev = x.shape[0], w._dev
+    y, ld = _output(out, M, N, w._buf, accumulate)
+    _launch(dev, "lb_mx_linear_grouped", MICROSCALED_FMT[w.fmt], x._codes, x._scales, x._t, M, K, x.offsets.data_ptr(), E,
+            w._codes, w._scales, w._t, N, _bias(bias, E * N, dev), 1 if accumulate else 0, y.data_ptr(), ld)
     return y
