@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 
 // One warp per token: k rounds of a warp-wide maximum over what is left; L logits per lane.
 template <int L>
-__device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int* hist) {
+__device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int* hist, int* list) {
   const int lane = threadIdx.x & 31;
   uint32_t key[L];
   float m = -INFINITY;
@@ -89,76 +89,113 @@ __device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int* his
   if (lane < p.k) {
     p.weights[t * p.k + lane] = sum > 0.f ? mine / sum : 0.f;
     p.experts[t * p.k + lane] = mine_e;
+    list[lane] = mine_e;
     atomicAdd(&hist[mine_e], 1);                     // whole numbers: the order does not matter
   }
 }
 
-// Chooses and counts: one block per chunk of TOK tokens.
+// Chooses for the tokens of a chunk: hist[e] = how often, list[i] = the expert of pair i (both in shared memory).
 template <int L>
-__global__ void __launch_bounds__(256) route_choose_kernel(const RouteParams p) {
-  extern __shared__ int hist[];
+__device__ __forceinline__ void choose_chunk(const RouteParams& p, int64_t t0, int* hist, int* list) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
   __syncthreads();
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOK;
-  for (int i = threadIdx.x >> 5; i < TOK && t0 + i < p.T; i += blockDim.x >> 5) choose<L>(p, t0 + i, hist);
+  for (int i = threadIdx.x >> 5; i < TOK && t0 + i < p.T; i += blockDim.x >> 5) choose<L>(p, t0 + i, hist, list + i * p.k);
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.E + e] = hist[e];
 }
 
-// Places: every block adds up the counts it needs, then one warp ranks its chunk's (token, j) in order.
-__global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p) {
-  extern __shared__ int next[];                      // [E] next free place of each expert for this chunk
-  const int chunks = gridDim.x;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+// Places the pairs of a chunk: next[e] = pairs of e in earlier chunks, next[E + e] = in all of them, list[i] = the expert of pair
+// i.  The first warp scans the experts, then ranks the pairs 32 at a time in order.
+__device__ __forceinline__ void place_chunk(const RouteParams& p, int64_t t0, int* next, const int* list, bool first) {
+  if (threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;
+  int run = 0;
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    const int n = e < p.E ? next[p.E + e] : 0;
+    int s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (e < p.E) {
+      next[e] += run + s - n;
+      if (first) p.offsets[e] = run + s - n;
+    }
+    run += __shfl_sync(0xffffffffu, s, 31);
+  }
+  if (first && lane == 0) p.offsets[p.E] = run;
+  __syncwarp();
+  const int64_t left = p.T - t0;
+  const int n = static_cast<int>(left < TOK ? left : TOK) * p.k;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    const bool in = i < n;
+    const int e = in ? list[i] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    const int place = in ? next[e] + rank : 0;
+    __syncwarp();
+    if (in && rank == 0) next[e] += __popc(same);
+    __syncwarp();
+    if (in) {
+      p.slots[t0 * p.k + i] = place;
+      p.rows[place] = static_cast<int>(t0 + i / p.k);
+    }
+  }
+}
+
+// T <= TOK: the whole routing in one block.
+template <int L>
+__global__ void __launch_bounds__(1024) route_small_kernel(const RouteParams p) {
+  extern __shared__ int sm[];                        // next [2 E], list [TOK k]
+  pdl_launch_dependents();
+  pdl_wait();
+  int* hist = sm + p.E;
+  int* list = sm + 2 * p.E;
+  choose_chunk<L>(p, 0, hist, list);
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) sm[e] = 0;
+  __syncthreads();
+  place_chunk(p, 0, sm, list, true);
+}
+
+// One block per chunk of TOK tokens.
+template <int L>
+__global__ void __launch_bounds__(1024) route_choose_kernel(const RouteParams p) {
+  extern __shared__ int sm[];                        // hist [E], list [TOK k]
+  pdl_launch_dependents();
+  pdl_wait();
+  choose_chunk<L>(p, static_cast<int64_t>(blockIdx.x) * TOK, sm, sm + p.E);
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.E + e] = sm[e];
+}
+
+// Every block adds up the counts of the chunks (a thread takes every P-th chunk of an expert), then places its own pairs.
+__global__ void __launch_bounds__(1024) route_place_kernel(const RouteParams p) {
+  extern __shared__ int sm[];                        // next [2 E], list [TOK k]
+  pdl_launch_dependents();
+  pdl_wait();
+  int* list = sm + 2 * p.E;
+  const int chunks = gridDim.x, mine = blockIdx.x;
+  const int64_t t0 = static_cast<int64_t>(mine) * TOK, left = p.T - t0;
+  for (int e = threadIdx.x; e < 2 * p.E; e += blockDim.x) sm[e] = 0;
+  __syncthreads();
+  const int P = blockDim.x / p.E > 0 ? blockDim.x / p.E : 1;
+  for (int i = threadIdx.x; i < P * p.E; i += blockDim.x) {
+    const int e = i % p.E;
     int before = 0, all = 0;
-    for (int c = 0; c < chunks; ++c) {
+#pragma unroll 8
+    for (int c = i / p.E; c < chunks; c += P) {
       const int n = p.counts[static_cast<int64_t>(c) * p.E + e];
-      before += c < static_cast<int>(blockIdx.x) ? n : 0;
+      before += c < mine ? n : 0;
       all += n;
     }
-    next[e] = before;
-    next[p.E + e] = all;
+    atomicAdd(&sm[e], before);                       // whole numbers: the order does not matter
+    atomicAdd(&sm[p.E + e], all);
   }
+  const int n = static_cast<int>(left < TOK ? left : TOK) * p.k;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) list[i] = p.experts[t0 * p.k + i];
   __syncthreads();
-  if (threadIdx.x < 32) {                            // exclusive scan over the experts
-    const int lane = threadIdx.x;
-    int run = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane;
-      const int n = e < p.E ? next[p.E + e] : 0;
-      int s = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += u;
-      }
-      if (e < p.E) {
-        next[e] += run + s - n;
-        if (blockIdx.x == 0) p.offsets[e] = run + s - n;
-      }
-      run += __shfl_sync(0xffffffffu, s, 31);
-    }
-    if (blockIdx.x == 0 && lane == 0) p.offsets[p.E] = run;
-    __syncwarp();
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOK;
-    const int64_t left = p.T - t0;
-    const int n = static_cast<int>(left < TOK ? left : TOK) * p.k;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      const bool in = i < n;
-      const int e = in ? p.experts[t0 * p.k + i] : -1;
-      const uint32_t same = __match_any_sync(0xffffffffu, e);
-      const int rank = __popc(same & ((1u << lane) - 1u));
-      const int place = in ? next[e] + rank : 0;
-      __syncwarp();
-      if (in && rank == 0) next[e] += __popc(same);
-      __syncwarp();
-      if (in) {
-        p.slots[t0 * p.k + i] = place;
-        p.rows[place] = static_cast<int>(t0 + i / p.k);
-      }
-    }
-  }
+  place_chunk(p, t0, sm, list, mine == 0);
 }
 
 struct CombineParams {
@@ -283,17 +320,20 @@ int lb_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld
   if (T == 0) return launched(cudaMemsetAsync(offsets, 0, (E + 1) * sizeof(int), st), "moe_route");
   moe::RouteParams p{logits, dtype, ldl, T, static_cast<int>(E), k, normalize ? 1 : 0, weights, experts, offsets, rows, slots,
                      static_cast<int*>(workspace)};
-  const unsigned g = static_cast<unsigned>(chunks);
-  const size_t sm = E * sizeof(int);
-  if (E <= 32) moe::route_choose_kernel<1><<<g, 256, sm, st>>>(p);
-  else if (E <= 64) moe::route_choose_kernel<2><<<g, 256, sm, st>>>(p);
-  else if (E <= 128) moe::route_choose_kernel<4><<<g, 256, sm, st>>>(p);
-  else if (E <= 256) moe::route_choose_kernel<8><<<g, 256, sm, st>>>(p);
-  else moe::route_choose_kernel<32><<<g, 256, sm, st>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return launched(e, "moe_route");
-  moe::route_place_kernel<<<g, 256, 2 * sm, st>>>(p);
-  return launched(cudaGetLastError(), "moe_route");
+  const int g = static_cast<int>(chunks);
+  const size_t sm = (2 * E + moe::TOK * k) * sizeof(int);
+  cudaError_t e;
+#define LB_MOE_ROUTE(L)                                                                                               \
+  e = g == 1 ? mx::launch_early(moe::route_small_kernel<L>, dim3(1), sm, st, p, 1024)                                       \
+             : mx::launch_early(moe::route_choose_kernel<L>, dim3(g), sm, st, p, 1024)
+  if (E <= 32) LB_MOE_ROUTE(1);
+  else if (E <= 64) LB_MOE_ROUTE(2);
+  else if (E <= 128) LB_MOE_ROUTE(4);
+  else if (E <= 256) LB_MOE_ROUTE(8);
+  else LB_MOE_ROUTE(32);
+#undef LB_MOE_ROUTE
+  if (e != cudaSuccess || g == 1) return launched(e, "moe_route");
+  return launched(mx::launch_early(moe::route_place_kernel, dim3(g), sm, st, p, 1024), "moe_route");
 }
 
 int lb_moe_combine(const void* z, int64_t rows, int64_t ldz, const float* weights, const int* slots, int64_t T, int k,
@@ -313,8 +353,8 @@ int lb_moe_combine(const void* z, int64_t rows, int64_t ldz, const float* weight
   int64_t blocks = (T * (vec ? H / 8 : H) + 255) / 256;
   if (blocks > static_cast<int64_t>(d->sms) * 16) blocks = static_cast<int64_t>(d->sms) * 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return launched(vec ? mx::launch_early(moe::combine_kernel<true>, static_cast<int>(blocks), 0, st, p)
-                      : mx::launch_early(moe::combine_kernel<false>, static_cast<int>(blocks), 0, st, p),
+  return launched(vec ? mx::launch_early(moe::combine_kernel<true>, dim3(static_cast<unsigned>(blocks)), 0, st, p)
+                      : mx::launch_early(moe::combine_kernel<false>, dim3(static_cast<unsigned>(blocks)), 0, st, p),
                   "moe_combine");
 }
 

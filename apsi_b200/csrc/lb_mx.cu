@@ -19,75 +19,85 @@ struct In {};
 template <>
 struct In<LB_DT_F32> {
   static constexpr int SIZE = 4;
-  static __device__ __forceinline__ float one(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
+  static __device__ __forceinline__ uint32_t bits(const void* p, int64_t i) { return static_cast<const uint32_t*>(p)[i]; }
 };
 template <>
 struct In<LB_DT_BF16> {
   static constexpr int SIZE = 2;
-  static __device__ __forceinline__ float one(const void* p, int64_t i) {
-    return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
-  }
+  static __device__ __forceinline__ uint32_t bits(const void* p, int64_t i) { return static_cast<const uint16_t*>(p)[i]; }
 };
 template <>
-struct In<LB_DT_F16> {
-  static constexpr int SIZE = 2;
-  static __device__ __forceinline__ float one(const void* p, int64_t i) { return __half2float(static_cast<const __half*>(p)[i]); }
-};
+struct In<LB_DT_F16> : In<LB_DT_BF16> {};
 
-// 16 values of a row from column c0 (zeros past K); vec: rows are aligned to 32 bytes (2), 16 (1) or their elements (0)
+// 16 values of a row as they lie in memory (zeros past K); vec: rows are aligned to 32 bytes (2), 16 (1) or elements (0)
 template <int DT>
-__device__ __forceinline__ void load16(const void* row, int64_t c0, int64_t K, int vec, float (&v)[16]) {
-  if (vec && c0 + 16 <= K) {
-    const char* p = static_cast<const char*>(row) + c0 * In<DT>::SIZE;
-    uint32_t w[DT == LB_DT_F32 ? 16 : 8];
+struct Raw {
+  static constexpr int NW = DT == LB_DT_F32 ? 16 : 8;
+  uint32_t w[NW];
+  __device__ __forceinline__ void load(const char* p, int64_t left, int vec) {   // left: values of the row from p on
+    if (vec && left >= 16) {
 #pragma unroll
-    for (int i = 0; i < In<DT>::SIZE / 2; ++i) {
-      if (vec == 2) {
-        ldg_nc_v8(p + 32 * i, *reinterpret_cast<uint32_t(*)[8]>(&w[8 * i]));
-      } else {
-        const uint4 a = ldg_nc_v4(p + 32 * i), b = ldg_nc_v4(p + 32 * i + 16);
-        w[8 * i] = a.x; w[8 * i + 1] = a.y; w[8 * i + 2] = a.z; w[8 * i + 3] = a.w;
-        w[8 * i + 4] = b.x; w[8 * i + 5] = b.y; w[8 * i + 6] = b.z; w[8 * i + 7] = b.w;
-      }
-    }
-    if constexpr (DT == LB_DT_F32) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (DT == LB_DT_BF16) {
-          v[2 * i] = __uint_as_float(w[i] << 16);
-          v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      for (int i = 0; i < NW / 8; ++i) {
+        if (vec == 2) {
+          ldg_nc_v8(p + 32 * i, *reinterpret_cast<uint32_t(*)[8]>(&w[8 * i]));
         } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
+          const uint4 a = ldg_nc_v4(p + 32 * i), b = ldg_nc_v4(p + 32 * i + 16);
+          w[8 * i] = a.x; w[8 * i + 1] = a.y; w[8 * i + 2] = a.z; w[8 * i + 3] = a.w;
+          w[8 * i + 4] = b.x; w[8 * i + 5] = b.y; w[8 * i + 6] = b.z; w[8 * i + 7] = b.w;
         }
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t u = i < left ? In<DT>::bits(p, i) : 0u;
+        if constexpr (DT == LB_DT_F32) w[i] = u;
+        else if (i & 1) w[i >> 1] |= u << 16;
+        else w[i >> 1] = u;
+      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c0 + i < K ? In<DT>::one(row, c0 + i) : 0.f;
   }
-}
-
-// Codes of y / s without 16 divisions.  y of a 16-bit type scaled by a power of two has at most 11 significant bits and
-// s 4, so a quotient that is no tie is at least 2^-11 away from every tie, relatively: y times the rounded inverse is
-// within 2^-22 of it, and rounding that to 16 significant bits puts every tie back on its place and moves nothing across one.
-__device__ __forceinline__ void codes_short(const float (&y)[16], float rs, uint32_t& lo, uint32_t& hi) {
-  float v[16];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float((__float_as_uint(y[i] * rs) + 0x80u) & 0xFFFFFF00u);
-  lo = e2m1_codes(v);
-  hi = e2m1_codes(v + 8);
-}
-// For any y: the codes of slightly more and slightly less than y / s (2^-20 either way, past the rounding of the inverse and
-// the product).  The quotient's code lies between; where the two differ (about one group of eight in 10^5 of random values)
-// the eight quotients are divided out.
+    for (int i = 0; i < NW; ++i) w[i] = 0u;
+  }
+  // bits of the largest |value| in float32 (not below infinity's if one is NaN or infinite)
+  __device__ __forceinline__ uint32_t amax() const {
+    if constexpr (DT == LB_DT_F32) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+      return m;
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i] & 0x7FFF7FFFu));
+      m = max(m >> 16, m & 0xFFFFu);
+      return DT == LB_DT_BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (DT == LB_DT_F32) return __uint_as_float(w[i]);
+    else if constexpr (DT == LB_DT_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    else {
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[i >> 1]);
+      return i & 1 ? __high2float(h) : __low2float(h);
+    }
+  }
+};
+
+// x / s for x with at most 11 significant bits and s with at most 4, good for rounding to a grid whose ties have at most
+// 5: c is slightly more than 1 / s (2^-20 of it, past the roundings of c and of the product), and cutting the product to 16
+// significant bits puts a quotient on a tie back on it.  Any other quotient is at least 2^-11 of a tie away from it and
+// stays on its side.
+__device__ __forceinline__ float cut(float x, float c) { return __uint_as_float(__float_as_uint(x * c) & 0xFFFFFF00u); }
+constexpr float MORE = 1.f + 0x1p-20f, LESS = 1.f - 0x1p-20f;
+
+// Eight codes of y / s for any y: the codes of slightly more and slightly less than it (2^-20 either way).  The quotient's code
+// lies between; where the two differ (about one group of eight in 10^5 of random values) the quotients are divided out.
 __device__ __forceinline__ uint32_t codes8_any(const float* y, float s, float rs) {
   float up[8], dn[8];
-  const float ru = rs * (1.f + 0x1p-20f), rd = rs * (1.f - 0x1p-20f);
+  const float ru = rs * MORE, rd = rs * LESS;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     up[i] = y[i] * ru;
@@ -99,6 +109,50 @@ __device__ __forceinline__ uint32_t codes8_any(const float* y, float s, float rs
   for (int i = 0; i < 8; ++i) up[i] = __fdiv_rn(y[i], s);
   return e2m1_codes(up);
 }
+
+// Rows over the grid: a warp takes 512 values of a row (16 a thread).  wpr = 1, 2, 4 or 8 warps of a block lie side by side
+// along a row and blockIdx.y counts groups of eight; block x takes `per` rows one after another, so nothing of the column is worked
+// out twice and a group is looked up where it ends.
+struct Rows {
+  int wpr_log, per;
+  __device__ __forceinline__ int first() const { return static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x >> (5 + wpr_log)); }
+  __device__ __forceinline__ int end(int64_t R) const {
+    const int64_t e = (static_cast<int64_t>(blockIdx.x) + 1) * per;
+    return static_cast<int>(e < R ? e : R);
+  }
+  __device__ __forceinline__ int step() const { return 8 >> wpr_log; }
+  __device__ __forceinline__ int64_t col() const {
+    return (static_cast<int64_t>(blockIdx.y) * 8 + ((threadIdx.x >> 5) & ((1 << wpr_log) - 1))) * 512 + (threadIdx.x & 31) * 16;
+  }
+};
+
+// The scales of rows that only grow, at one block column: where row r's lie (null: it is in no group).
+struct Walk {
+  uint8_t* col;                                // the column's place in the first row block
+  int64_t block;                               // bytes of a row block
+  int lo, hi;                                  // the current group's rows, and its first row block
+  int64_t blk;
+  __device__ __forceinline__ Walk(const uint8_t* scales, int64_t c, int64_t acols, const Groups& g)
+      : col(const_cast<uint8_t*>(scales) + (c >> 2) * 512 + (c & 3)), block(acols * 512), lo(0), hi(g.G ? 0 : 0x7FFFFFFF), blk(0) {}
+  __device__ __forceinline__ uint8_t* at(const Groups& g, const int* off, const int* base, int gblocks, int r) {
+    if (r >= hi) {
+      if (g.per > 0) {
+        const int e = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(g.per));
+        lo = e * static_cast<int>(g.per);
+        hi = lo + static_cast<int>(g.per);
+        blk = static_cast<int64_t>(e) * gblocks;
+      } else {
+        const int e = group_of(off, g.G, r);
+        if (e < 0) return nullptr;
+        lo = off[e];
+        hi = off[e + 1];
+        blk = base[e];
+      }
+    }
+    const int rg = r - lo;
+    return col + (blk + (rg >> 7)) * block + ((rg & 31) * 16 + ((rg >> 5) & 3) * 4);
+  }
+};
 
 struct QuantParams {
   const void* x;            // [Rin, K], row stride ldx
@@ -112,6 +166,7 @@ struct QuantParams {
   uint8_t* codes;
   uint8_t* scales;
   int vec;
+  Rows over;
 };
 
 // The smallest power of two t with amax / t <= 448 * 6 = 1.3125 * 2^11 (1 for a zero tensor), so that dividing
@@ -124,30 +179,12 @@ __device__ __forceinline__ float auto_scale(float amax) {
   return pow2f(e < -126 ? -126 : e);
 }
 
-// Where row r lies: its place in its group and the group's first row block (false: it is in no group).
-__device__ __forceinline__ bool place_of(const Groups& g, const int* off, const int* base, int64_t gblocks, int64_t r,
-                                         int64_t& rg, int64_t& blk0) {
-  rg = r;
-  blk0 = 0;
-  if (g.G == 0) return true;
-  int64_t e;
-  if (g.per > 0) {
-    e = static_cast<uint32_t>(r) / static_cast<uint32_t>(g.per);
-    rg = r - e * g.per;
-    blk0 = e * gblocks;
-  } else {
-    e = group_of(off, g.G, r);
-    if (e < 0) return false;
-    rg = r - off[e];
-    blk0 = base[e];
-  }
-  return true;
-}
+constexpr int QUANT_BLOCKS = 4, DEQUANT_BLOCKS = 6;   // resident on an SM; the grid is one wave of them
 
-// One thread per 16 values, a warp per 512 values of one row.  Memory-bound: 32-byte loads, whole sectors; the next row's
-// index is on its way while this row is rounded.
+// Memory-bound in its bytes; in instructions about 6 a value for 16-bit types, so the divisions are taken out (cut, codes8_any)
+// and the maximum is taken on pairs.  The next row's values and the index after it are on their way while a row is rounded.
 template <int FMT, int DT>
-__global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
+__global__ void __launch_bounds__(256, QUANT_BLOCKS) quant_kernel(const QuantParams p) {
   extern __shared__ int sm[];
   pdl_launch_dependents();
   pdl_wait();
@@ -165,7 +202,7 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (lane == 0) {
           s_t = auto_scale(m);
-          if (blockIdx.x == 0) *p.t_out = s_t;
+          if (blockIdx.x == 0 && blockIdx.y == 0) *p.t_out = s_t;
         }
       }
     } else if (threadIdx.x == 0) {
@@ -174,43 +211,41 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
     __syncthreads();
   }
   const float t = FMT == LB_FMT_NVFP4 ? s_t : 1.f;
-  // dividing by a power of two is multiplying by its inverse, exactly
-  const bool pow2 = FMT == LB_FMT_NVFP4 && (__float_as_uint(t) & 0x807FFFFFu) == 0 && t >= pow2f(-126) && t <= pow2f(126);
+  // dividing by a power of two is multiplying by its inverse, exactly (within 2^+-100 also where it meets a block's scale)
+  const bool pow2 = FMT == LB_FMT_NVFP4 && (__float_as_uint(t) & 0x807FFFFFu) == 0 && t >= pow2f(-100) && t <= pow2f(100);
   const float inv = 1.0f / t;
-  const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K);
-  const uint32_t segs = static_cast<uint32_t>((p.K + 511) / 512);
-  const int64_t nseg = p.R * segs, step = static_cast<int64_t>(gridDim.x) * 8;
-  const int64_t gblocks = p.g.per > 0 ? (p.g.per + 127) / 128 : 0;
-  auto split = [&](int64_t w, int64_t& r, int64_t& c) {          // warp item -> row, first column
-    r = nseg <= 0xFFFFFFFFll ? static_cast<uint32_t>(w) / segs : w / segs;
-    c = (w - r * segs) * 512;
-  };
-  int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), r, c0;
-  split(w < nseg ? w : 0, r, c0);
-  int64_t src = p.rows && w < nseg ? p.rows[r] : r;
-  while (w < nseg) {
-    const int64_t wn = w + step;
-    int64_t rn, cn;
-    split(wn < nseg ? wn : 0, rn, cn);
-    c0 += lane * 16;
-    float v[16];
+  const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K), c0 = p.over.col();
+  const int gblocks = p.g.per > 0 ? static_cast<int>((p.g.per + 127) / 128) : 0;
+  constexpr int PER = FMT == LB_FMT_MXFP4 ? 2 : 1;               // threads of a block
+  const int64_t c = c0 / block_of(FMT);
+  const bool put_scale = lane % (4 * PER) == 0 && c < acols * 4, put_codes = c0 < rb * 2;
+  const int step = p.over.step(), end = p.over.end(p.R);
+  int r = p.over.first();
+  if (r >= end) return;
+  const char* const xc = static_cast<const char*>(p.x) + c0 * In<DT>::SIZE;
+  const int64_t xrow = p.ldx * In<DT>::SIZE, left = p.K - c0;
+  auto source = [&](int i) { return p.rows && i < end ? p.rows[i] : i; };
+  auto load = [&](int src) {
+    Raw<DT> x;
     if (src >= 0 && src < p.Rin) {
-      load16<DT>(static_cast<const char*>(p.x) + src * p.ldx * In<DT>::SIZE, c0, p.K, p.vec, v);
+      x.load(xc + src * xrow, left, p.vec);
     } else {                                                     // no such row: zeros, and the error word says so
       if (lane == 0) atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      x.zero();
     }
-    const int64_t srcn = p.rows && wn < nseg ? p.rows[rn] : rn;
-    int64_t rg, blk0;
-    const bool in = place_of(p.g, off, base, gblocks, r, rg, blk0);   // rows of no group are left alone
-    uint32_t am = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-      am = b > am ? b : am;
-    }
-    uint32_t byte, lo, hi;
+    return x;
+  };
+  int src = source(r + step);
+  Raw<DT> next = load(source(r));
+  Walk walk(p.scales, c, acols, p.g);
+  uint8_t* cp = p.codes + r * rb + c0 / 2;
+  for (; r < end; r += step, cp += step * rb) {
+    const Raw<DT> x = next;
+    if (r + step < end) next = load(src);
+    src = source(r + 2 * step);
+    uint8_t* const sp = walk.at(p.g, off, base, gblocks, r);     // rows of no group are left alone
+    uint32_t am = x.amax(), byte, lo, hi;
+    float v[16];
     if (FMT == LB_FMT_MXFP4) {
       const uint32_t o = __shfl_xor_sync(0xffffffffu, am, 1);
       am = o > am ? o : am;
@@ -218,64 +253,68 @@ __global__ void __launch_bounds__(256) quant_kernel(const QuantParams p) {
       byte = f == 255u ? 255u : (f > 2u ? f - 2u : 0u);
       const float mul = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] *= mul;
+      for (int i = 0; i < 16; ++i) v[i] = x[i] * mul;
       lo = e2m1_codes(v);
       hi = e2m1_codes(v + 8);
     } else {
       const bool bad = am >= 0x7F800000u;
-      float a = __uint_as_float(am);
-      a = pow2 ? a * inv : __fdiv_rn(a, t);
-      byte = bad ? 0x7Fu : e4m3_byte(__fdiv_rn(a, 6.0f));
-      const float s = e4m3_value(byte), rs = byte == 0u || bad ? 0.f : 1.0f / s;   // no scale: zeros with their signs
-      if (pow2) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= inv;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __fdiv_rn(v[i], t);
-      }
       if (DT != LB_DT_F32 && pow2) {
-        codes_short(v, rs, lo, hi);
+        byte = bad ? 0x7Fu : e4m3_byte(cut(__uint_as_float(am) * inv, (1.f / 6.f) * MORE));
+        // no scale: zeros with their signs
+        const float k = byte == 0u || bad ? 0.f : __fdividef(MORE, e4m3_value(byte)) * inv;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = cut(x[i], k);
+        lo = e2m1_codes(v);
+        hi = e2m1_codes(v + 8);
       } else {
+        float a = __uint_as_float(am);
+        a = pow2 ? a * inv : __fdiv_rn(a, t);
+        byte = bad ? 0x7Fu : e4m3_byte(__fdiv_rn(a, 6.0f));
+        const float s = e4m3_value(byte), rs = byte == 0u || bad ? 0.f : __fdividef(1.0f, s);
+        if (pow2) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = x[i] * inv;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = __fdiv_rn(x[i], t);
+        }
         lo = codes8_any(v, s, rs);
         hi = codes8_any(v + 8, s, rs);
       }
     }
-    if (in && c0 < rb * 2) *reinterpret_cast<uint2*>(p.codes + r * rb + c0 / 2) = make_uint2(lo, hi);
+    if (sp && put_codes) *reinterpret_cast<uint2*>(cp) = make_uint2(lo, hi);
     // four scale bytes of neighbouring blocks make one word
-    constexpr int PER = FMT == LB_FMT_MXFP4 ? 2 : 1;
     uint32_t word = byte;
     word |= __shfl_down_sync(0xffffffffu, word, PER) << 8;
     word = (word & 0xFFFFu) | (__shfl_down_sync(0xffffffffu, word, 2 * PER) << 16);
-    const int64_t c = c0 / block_of(FMT);
-    if (in && lane % (4 * PER) == 0 && c < acols * 4)
-      *reinterpret_cast<uint32_t*>(p.scales + blk0 * acols * 512 + scale_at(rg, c, acols)) = word;
-    w = wn;
-    r = rn;
-    c0 = cn;
-    src = srcn;
+    if (sp && put_scale) *reinterpret_cast<uint32_t*>(sp) = word;
   }
 }
 
 // Partial maxima of |x| over finite values, one per block.
 template <int DT>
-__global__ void __launch_bounds__(256) amax_kernel(const void* __restrict__ x, int64_t R, int64_t K, int64_t ldx, int vec,
-                                                   float* __restrict__ part) {
+__global__ void __launch_bounds__(256) amax_kernel(const QuantParams p) {
   __shared__ uint32_t red[8];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t segs = (K + 511) / 512, nseg = R * segs;
+  const int64_t c0 = p.over.col();
+  const char* const xc = static_cast<const char*>(p.x) + c0 * In<DT>::SIZE;
+  const int step = p.over.step(), end = p.over.end(p.Rin);
   uint32_t am = 0;
-  for (int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < nseg;
-       w += static_cast<int64_t>(gridDim.x) * 8) {
-    const int64_t r = w / segs;
-    float v[16];
-    load16<DT>(static_cast<const char*>(x) + r * ldx * In<DT>::SIZE, (w - r * segs) * 512 + lane * 16, K, vec, v);
+#pragma unroll 4
+  for (int r = p.over.first(); r < end; r += step) {
+    Raw<DT> x;
+    x.load(xc + r * (p.ldx * In<DT>::SIZE), p.K - c0, p.vec);
+    const uint32_t m = x.amax();
+    if (m < 0x7F800000u) {
+      am = max(am, m);
+    } else {                                                     // look at the finite ones
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-      am = b > am && b < 0x7F800000u ? b : am;
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t b = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+        am = b > am && b < 0x7F800000u ? b : am;
+      }
     }
   }
   am = __reduce_max_sync(0xffffffffu, am);
@@ -284,7 +323,7 @@ __global__ void __launch_bounds__(256) amax_kernel(const void* __restrict__ x, i
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) am = red[i] > am ? red[i] : am;
-    part[blockIdx.x] = __uint_as_float(am);
+    const_cast<float*>(p.part)[blockIdx.y * gridDim.x + blockIdx.x] = __uint_as_float(am);
   }
 }
 
@@ -295,12 +334,13 @@ struct DequantParams {
   int64_t R, K, ldo;
   Groups g;
   void* out;
-  int vec;                  // as load16's
+  int vec;                  // as Raw::load's
+  Rows over;
 };
 
 // One thread per 16 values.
 template <int FMT, int ODT>
-__global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) {
+__global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const DequantParams p) {
   extern __shared__ int sm[];
   pdl_launch_dependents();
   pdl_wait();
@@ -308,19 +348,35 @@ __global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) 
   int* base = sm + p.g.G + 1;
   if (p.g.G > 0 && p.g.per == 0) load_groups(p.g, p.R, off, base);
   const float t = FMT == LB_FMT_NVFP4 && p.t ? *p.t : 1.f;
-  const int lane = threadIdx.x & 31;
-  const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K);
-  const uint32_t segs = static_cast<uint32_t>((p.K + 511) / 512);
-  const int64_t nseg = p.R * segs;
-  const int64_t gblocks = p.g.per > 0 ? (p.g.per + 127) / 128 : 0;
-  for (int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < nseg;
-       w += static_cast<int64_t>(gridDim.x) * 8) {
-    const int64_t r = nseg <= 0xFFFFFFFFll ? static_cast<uint32_t>(w) / segs : w / segs;
-    const int64_t c0 = (w - r * segs) * 512 + lane * 16;
-    int64_t rg, blk0;
-    if (c0 >= p.K || !place_of(p.g, off, base, gblocks, r, rg, blk0)) continue;
-    const uint2 q = *reinterpret_cast<const uint2*>(p.codes + r * rb + c0 / 2);
-    const float s = scale_value<FMT>(p.scales[blk0 * acols * 512 + scale_at(rg, c0 / block_of(FMT), acols)]);
+  const bool pow2 = FMT == LB_FMT_NVFP4 && (__float_as_uint(t) & 0x807FFFFFu) == 0 && t >= pow2f(-100) && t <= pow2f(100);
+  const int64_t rb = row_bytes(p.K), acols = atom_cols(FMT, p.K), c0 = p.over.col(), c = c0 / block_of(FMT);
+  const int gblocks = p.g.per > 0 ? static_cast<int>((p.g.per + 127) / 128) : 0;
+  const int step = p.over.step(), end = p.over.end(p.R);
+  constexpr int NW = ODT == LB_DT_F32 ? 16 : 8, ES = ODT == LB_DT_F32 ? 4 : 2;
+  if (c0 >= p.K) return;
+  Walk walk(p.scales, c, acols, p.g);
+  struct Packed { uint2 q; uint32_t s; bool in; };
+  auto load = [&](int r) {                     // codes and scale byte of a row
+    Packed u{make_uint2(0u, 0u), 0u, false};
+    if (r < end) {
+      if (const uint8_t* sp = walk.at(p.g, off, base, gblocks, r)) {
+        u.q = *reinterpret_cast<const uint2*>(p.codes + r * rb + c0 / 2);
+        u.s = *sp;
+        u.in = true;
+      }
+    }
+    return u;
+  };
+  int r = p.over.first();
+  const bool whole = p.vec && c0 + 16 <= p.K;
+  Packed next = load(r);
+  for (; r < end; r += step) {
+    const Packed now = next;
+    next = load(r + step);
+    if (!now.in) continue;
+    const uint2 q = now.q;
+    float s = scale_value<FMT>(now.s);
+    if (pow2) s *= t;                          // exact, so the same as multiplying by it last
     uint32_t h[8];
     {
       uint32_t a[4], b[4];
@@ -336,11 +392,10 @@ __global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) 
       v[2 * i] = f.x * s;                      // exact: 2 significant bits times a power of two or 4 bits
       v[2 * i + 1] = f.y * s;
     }
-    if (FMT == LB_FMT_NVFP4) {
+    if (FMT == LB_FMT_NVFP4 && !pow2) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= t;
     }
-    constexpr int NW = ODT == LB_DT_F32 ? 16 : 8, ES = ODT == LB_DT_F32 ? 4 : 2;
     uint32_t u[NW];
     if constexpr (ODT == LB_DT_F32) {
 #pragma unroll
@@ -358,7 +413,7 @@ __global__ void __launch_bounds__(256) dequant_kernel_mx(const DequantParams p) 
       }
     }
     char* o = static_cast<char*>(p.out) + (r * p.ldo + c0) * ES;
-    if (p.vec && c0 + 16 <= p.K) {
+    if (whole) {
 #pragma unroll
       for (int i = 0; i < NW / 8; ++i) {
         if (p.vec == 2) {
@@ -401,9 +456,17 @@ __global__ void __launch_bounds__(256) scales_kernel(uint8_t* __restrict__ plain
 }
 
 constexpr int MAX_PARTS = LB_MX_PARTIALS;
-static int quant_blocks(int64_t R, int64_t K, int sms) {
-  const int64_t nseg = R * ((K + 511) / 512), b = (nseg + 7) / 8;
-  return static_cast<int>(b < static_cast<int64_t>(sms) * 8 ? b : static_cast<int64_t>(sms) * 8);
+// At most `most` blocks over R rows of K values
+static dim3 over_rows(int64_t R, int64_t K, int64_t most, Rows* over) {
+  const int64_t segs = (K + 511) / 512;
+  over->wpr_log = segs > 4 ? 3 : (segs > 2 ? 2 : (segs > 1 ? 1 : 0));
+  const int64_t gy = (segs + 7) / 8, rpb = 8 >> over->wpr_log;
+  int64_t gx = (R + rpb - 1) / rpb;
+  if (gx > most / gy) gx = most / gy;
+  if (gx < 1) gx = 1;
+  over->per = static_cast<int>(((R + gx - 1) / gx + rpb - 1) / rpb * rpb);
+  gx = (R + over->per - 1) / over->per;
+  return dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
 }
 // 2: rows are 32-byte aligned, 1: 16, 0: neither
 static int row_vec(const void* p, int64_t ld, int es) {
@@ -411,10 +474,10 @@ static int row_vec(const void* p, int64_t ld, int es) {
 }
 // A launch that may begin while the kernel before it ends (it waits for that one before it touches memory).
 template <typename P>
-static cudaError_t launch_early(void (*kernel)(P), int blocks, size_t smem, cudaStream_t st, const P& p) {
+static cudaError_t launch_early(void (*kernel)(P), dim3 blocks, size_t smem, cudaStream_t st, const P& p, int threads = 256) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = blocks;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at;
@@ -461,7 +524,8 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
   if (x_dtype != LB_DT_F32 && x_dtype != LB_DT_BF16 && x_dtype != LB_DT_F16)
     return fail(LB_E_ARG, "lb_mx_quant: x_dtype must be LB_DT_F32, LB_DT_BF16 or LB_DT_F16");
   if (Rin < 0 || R < 0 || K <= 0 || ldx < K) return fail(LB_E_ARG, "lb_mx_quant: bad sizes (K positive, ldx >= K)");
-  if (Rin > 0x7FFFFFFF || R > 0x7FFFFFFF) return fail(LB_E_ARG, "lb_mx_quant: at most 2^31 - 1 rows");
+  if (Rin > 0x7FFFFF00 || R > 0x7FFFFF00 || K > 0x7FFFFFF)
+    return fail(LB_E_ARG, "lb_mx_quant: at most 2^31 - 256 rows of 2^27 - 1 values");
   if (!rows && R != Rin) return fail(LB_E_ARG, "lb_mx_quant: R must be the rows of x when none are chosen");
   int r = mx::check_groups("lb_mx_quant", offsets, G, per, R);
   if (r) return r;
@@ -484,22 +548,21 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
   p.part = nullptr; p.t_out = nullptr; p.nparts = 0;
   p.codes = codes; p.scales = scales;
   p.vec = mx::row_vec(x, ldx, es);
+  cudaError_t e;
   if (fmt == LB_FMT_NVFP4 && !tensor_scale) {
-    int nb = mx::quant_blocks(Rin, K, d->sms);
-    if (nb > mx::MAX_PARTS) nb = mx::MAX_PARTS;
-    if (nb < 1) nb = 1;
+    const int64_t segs = (K + 511) / 512;
+    if (segs > 8 * mx::MAX_PARTS) return fail(LB_E_UNSUPPORTED, "lb_mx_quant: K above %d needs tensor_scale", 8 * 512 * mx::MAX_PARTS);
+    const dim3 nb = mx::over_rows(Rin > 0 ? Rin : 1, K, mx::MAX_PARTS, &p.over);
     p.part = auto_scale + 1;
     p.t_out = auto_scale;
-    p.nparts = nb;
-    if (x_dtype == LB_DT_F32) mx::amax_kernel<LB_DT_F32><<<nb, 256, 0, st>>>(x, Rin, K, ldx, p.vec, auto_scale + 1);
-    else if (x_dtype == LB_DT_BF16) mx::amax_kernel<LB_DT_BF16><<<nb, 256, 0, st>>>(x, Rin, K, ldx, p.vec, auto_scale + 1);
-    else mx::amax_kernel<LB_DT_F16><<<nb, 256, 0, st>>>(x, Rin, K, ldx, p.vec, auto_scale + 1);
-    cudaError_t e = cudaGetLastError();
+    p.nparts = static_cast<int>(nb.x * nb.y);
+    e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::amax_kernel<LB_DT_F32>, nb, 0, st, p)
+        : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::amax_kernel<LB_DT_BF16>, nb, 0, st, p)
+                                : mx::launch_early(mx::amax_kernel<LB_DT_F16>, nb, 0, st, p);
     if (e != cudaSuccess) return launched(e, "mx_amax");
   }
-  const int blocks = mx::quant_blocks(R, K, d->sms);
+  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::QUANT_BLOCKS, &p.over);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
-  cudaError_t e;
 #define LB_MX_QUANT(F)                                                                                              \
   e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::quant_kernel<F, LB_DT_F32>, blocks, sm, st, p)                 \
       : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::quant_kernel<F, LB_DT_BF16>, blocks, sm, st, p)                \
@@ -515,7 +578,7 @@ int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const fl
   if (!mx::is_mx(fmt)) return fail(LB_E_ARG, "lb_mx_dequant: format %d is not microscaled", fmt);
   if (out_dtype != LB_DT_F32 && out_dtype != LB_DT_BF16 && out_dtype != LB_DT_F16)
     return fail(LB_E_ARG, "lb_mx_dequant: out_dtype must be LB_DT_F32, LB_DT_BF16 or LB_DT_F16");
-  if (R < 0 || K <= 0 || ldo < K || R > 0x7FFFFFFF) return fail(LB_E_ARG, "lb_mx_dequant: bad sizes");
+  if (R < 0 || K <= 0 || ldo < K || R > 0x7FFFFF00 || K > 0x7FFFFFF) return fail(LB_E_ARG, "lb_mx_dequant: bad sizes");
   int r = mx::check_groups("lb_mx_dequant", offsets, G, per, R);
   if (r) return r;
   if (R == 0) return LB_OK;
@@ -526,8 +589,8 @@ int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const fl
   DevInfo* d;
   if ((r = current(&d))) return r;
   mx::DequantParams p{codes, scales, tensor_scale, R, K, ldo, {offsets, static_cast<int>(G), per}, out,
-                      mx::row_vec(out, ldo, es)};
-  const int blocks = mx::quant_blocks(R, K, d->sms);
+                      mx::row_vec(out, ldo, es), {0, 0}};
+  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::DEQUANT_BLOCKS, &p.over);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
