@@ -17,7 +17,7 @@
 //
 // Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales, 8.. epilogue (4 or 8 warps; warp w reads lanes
 // 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
-// takes it into registers as bf16 at once and stores while the next tile's products run.
+// takes it into registers at once and converts and stores while the next tile's products run.
 //
 // Few units (decode, small layers): a cluster of S CTAs splits K; each leaves its float32 tile in its own shared
 // memory and every CTA adds its share of the columns over the cluster in rank order: one launch, no workspace, the
@@ -360,27 +360,30 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
     // ------------------------------------------------------------------ MMA issuer
     if (half == 0 && elect_one()) {
       uint32_t it = 0, tc = 0;
+      const uint64_t da0 = smem_desc_sw128(smem_u32(as)), db0 = smem_desc_sw128(smem_u32(bs));   // + 16-byte units
+      const int last = static_cast<int>(((p.K + 31) / 32 * 32 - (static_cast<int64_t>(p.ksteps) - 1) * 256 + 63) >> 6);
       for (int u = u0; u < units; u += du, ++tc) {
         const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
         const int N = SWAP ? BT : (t.tn + 15) / 16 * 16;
+        const uint32_t id0 = idesc_mx<FMT, CG>(N, 0), id2 = idesc_mx<FMT, CG>(N, 2);
         const uint32_t b = tc % C::ACCS;
         if (tc >= C::ACCS) mbar_wait(&acc_empty[b], ((tc / C::ACCS) - 1) & 1, abort_v);
         tc_fence_after();
         const uint32_t d = tmem + b * BT;
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
-          mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
+          // the warps that stored the scales waited for the stage's copies, so this wait stands for both
           mbar_wait(&sf_full[slot], (it / STAGES) & 1, abort_v);
           tc_fence_after();
-          const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
-          const uint32_t aa = smem_u32(as + slot * A_BYTES), ab = smem_u32(bs + slot * C::B_BYTES);
-          const int64_t kleft = (p.K + 31) / 32 * 32 - static_cast<int64_t>(ks) * 256;
-          const int nk = kleft >= 256 ? 4 : static_cast<int>((kleft + 63) >> 6);
-          for (int kk = 0; kk < nk; ++kk) {
-            const int a = FMT == LB_FMT_MXFP4 ? kk >> 1 : kk;
-            const uint32_t sf = FMT == LB_FMT_MXFP4 ? (kk & 1) * 2 : 0;
-            tc_mma_mx<FMT, CG>(d, smem_desc_sw128(aa + kk * 32), smem_desc_sw128(ab + kk * 32), idesc_mx<FMT, CG>(N, sf),
-                               ca + a * 4, cb + a * (4 * C::NB) + (SWAP ? 0 : t.toff >> 5), (ks > k0 || kk > 0) ? 1u : 0u);
+          const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4 + (SWAP ? 0 : t.toff >> 5);
+          const uint64_t da = da0 + slot * (A_BYTES >> 4), db = db0 + slot * (C::B_BYTES >> 4);
+          const int nk = ks + 1 < p.ksteps ? 4 : last;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            if (kk >= nk) break;
+            const int a = FMT == LB_FMT_MXFP4 ? kk >> 1 : kk;     // scale atom; mxf4 takes half of its columns
+            tc_mma_mx<FMT, CG>(d, da + kk * 2, db + kk * 2, FMT == LB_FMT_MXFP4 && (kk & 1) ? id2 : id0, ca + a * 4,
+                               cb + a * (4 * C::NB), (ks > k0 || kk > 0) ? 1u : 0u);
           }
           tc_commit_all<CG>(&empty[slot]);
         }
@@ -470,28 +473,39 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
       } else {
         const int64_t m = t.tok0 + half * 128 + rloc;
         const bool ok = half * 128 + rloc < t.tn;
-        uint32_t o[HALF / 2];                                    // this row's part as bf16 pairs
         const int cl = cols - h * HALF;                          // columns of the part that exist
         uint16_t* yr = p.y + m * p.ldy + t.n0 + h * HALF;
         const uint16_t* br = p.bias ? p.bias + t.e * p.N + t.n0 + h * HALF : nullptr;
+        // 64 columns at a time: packed as bf16, the first leave room for the last, and the accumulator is free (the next tile's
+        // products begin) before those are converted and anything is stored
+        uint32_t o[HALF / 2], v[2][32];
+        auto pack = [&](int g) {
 #pragma unroll
-        for (int c0 = 0; c0 < HALF; c0 += 32) {
-          uint32_t v[32];
-          tmem_ld_x32(d + c0, v);
-          tc_wait_ld();
+          for (int i = 0; i < 2; ++i) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-          if (br) add_row(v, br + c0, cl - c0, p.vec & VEC_BIAS);
-          if (p.acc && ok) add_row(v, yr + c0, cl - c0, p.vec & VEC_Y16);
+            for (int j = 0; j < 32; ++j) v[i][j] = __float_as_uint(__uint_as_float(v[i][j]) * alpha);
+            const int c = 64 * g + 32 * i;
+            if (br) add_row(v[i], br + c, cl - c, p.vec & VEC_BIAS);
+            if (p.acc && ok) add_row(v[i], yr + c, cl - c, p.vec & VEC_Y16);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const __nv_bfloat162 bb = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-            o[c0 / 2 + j] = *reinterpret_cast<const uint32_t*>(&bb);
+            for (int j = 0; j < 16; ++j) {
+              const __nv_bfloat162 bb = __floats2bfloat162_rn(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1]));
+              o[c / 2 + j] = *reinterpret_cast<const uint32_t*>(&bb);
+            }
           }
+        };
+#pragma unroll
+        for (int g = 0; g < HALF / 64; ++g) {
+          tmem_ld_x32(d + 64 * g, v[0]);
+          tmem_ld_x32(d + 64 * g + 32, v[1]);
+          tc_wait_ld();
+          if (g == HALF / 64 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_first<CG>(&acc_empty[b]);
+          }
+          pack(g);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_first<CG>(&acc_empty[b]);          // the accumulator is free; the stores run on
         if (ok) {
           if ((p.vec & VEC_Y32) && cl >= HALF) {                 // whole 32-byte sectors
 #pragma unroll
