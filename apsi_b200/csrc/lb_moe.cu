@@ -17,7 +17,6 @@ constexpr int TOK = 64;                 // tokens of a chunk: one block ranks on
 
 struct RouteParams {
   const void* logits;
-  int dt;
   int64_t ldl, T;
   int E, k, normalize;
   float* weights;
@@ -28,11 +27,11 @@ struct RouteParams {
   int* counts;                          // [chunks][E]
 };
 
-__device__ __forceinline__ float logit(const RouteParams& p, int64_t t, int e) {
-  const int64_t i = t * p.ldl + e;
+template <int DT>
+__device__ __forceinline__ float logit(const RouteParams& p, int64_t i) {
   float v;
-  if (p.dt == LB_DT_F32) v = static_cast<const float*>(p.logits)[i];
-  else if (p.dt == LB_DT_BF16) v = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.logits)[i]) << 16);
+  if (DT == LB_DT_F32) v = static_cast<const float*>(p.logits)[i];
+  else if (DT == LB_DT_BF16) v = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.logits)[i]) << 16);
   else v = __half2float(static_cast<const __half*>(p.logits)[i]);
   return v == v ? v : -INFINITY;
 }
@@ -42,52 +41,52 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One warp per token: k rounds of a warp-wide maximum over what is left; L logits per lane.
-template <int L>
+// One warp per token: k rounds of a warp-wide maximum over what is left (the order of floats as unsigned numbers, the lowest
+// index of equals), L logits per lane; lane j keeps choice j, and the weights are worked out once at the end.
+template <int L, int DT>
 __device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int* hist, int* list) {
   const int lane = threadIdx.x & 31;
-  uint32_t key[L];
-  float m = -INFINITY;
+  uint32_t key[L], most = 0;
+  const int64_t row = t * p.ldl + lane;
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     const int e = i * 32 + lane;
-    const float v = e < p.E ? logit(p, t, e) : -INFINITY;
-    key[i] = e < p.E ? order_key(v) : 0u;            // 0: none (every float's key is above it)
-    m = fmaxf(m, v);
+    key[i] = e < p.E ? order_key(logit<DT>(p, row + i * 32)) : 0u;   // 0: none (every float's key is above it)
+    most = key[i] > most ? key[i] : most;
   }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  auto weight = [&](uint32_t u) {
-    const float v = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
-    return m == -INFINITY ? 0.f : (v == m ? 1.f : expf(v - m));
-  };
+  const uint32_t top0 = __reduce_max_sync(0xffffffffu, most);
+  auto value = [](uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); };
+  const float m = value(top0);
+  auto weight = [&](uint32_t u) { return u == top0 ? 1.f : expf(value(u) - m); };
   float sum = 0.f;
   if (!p.normalize) {
 #pragma unroll
     for (int i = 0; i < L; ++i) if (key[i]) sum += weight(key[i]);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  float mine = 0.f;                                  // lane j holds choice j
+  uint32_t mine = 0;
   int mine_e = 0;
   for (int j = 0; j < p.k; ++j) {
-    uint32_t best = 0;
-    int at = 0;
+    const uint32_t top = j ? __reduce_max_sync(0xffffffffu, most) : top0;
+    uint32_t e = 0xFFFFFFFFu;                        // this lane's first place with it
 #pragma unroll
-    for (int i = 0; i < L; ++i)
-      if (key[i] > best) { best = key[i]; at = i; }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFFFFFu);
-    if ((e & 31u) == static_cast<uint32_t>(lane)) {
+    for (int i = L - 1; i >= 0; --i) if (key[i] == top) e = i * 32 + lane;
+    e = __reduce_min_sync(0xffffffffu, e);
+    if ((e & 31u) == static_cast<uint32_t>(lane)) {  // taken: the lane's next best
+      most = 0;
 #pragma unroll
-      for (int i = 0; i < L; ++i) if (i == static_cast<int>(e >> 5)) key[i] = 0;
+      for (int i = 0; i < L; ++i) {
+        if (i == static_cast<int>(e >> 5)) key[i] = 0;
+        most = key[i] > most ? key[i] : most;
+      }
     }
-    const float w = weight(top);
-    if (p.normalize) sum += w;
-    if (lane == j) { mine = w; mine_e = static_cast<int>(e); }
+    if (lane == j) { mine = top; mine_e = static_cast<int>(e); }
   }
+  const float w = lane < p.k ? weight(mine) : 0.f;
+  if (p.normalize) sum = w;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane < p.k) {
-    p.weights[t * p.k + lane] = sum > 0.f ? mine / sum : 0.f;
+    p.weights[t * p.k + lane] = m == -INFINITY ? 0.f : w / sum;
     p.experts[t * p.k + lane] = mine_e;
     list[lane] = mine_e;
     atomicAdd(&hist[mine_e], 1);                     // whole numbers: the order does not matter
@@ -95,11 +94,11 @@ __device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int* his
 }
 
 // Chooses for the tokens of a chunk: hist[e] = how often, list[i] = the expert of pair i (both in shared memory).
-template <int L>
+template <int L, int DT>
 __device__ __forceinline__ void choose_chunk(const RouteParams& p, int64_t t0, int* hist, int* list) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x >> 5; i < TOK && t0 + i < p.T; i += blockDim.x >> 5) choose<L>(p, t0 + i, hist, list + i * p.k);
+  for (int i = threadIdx.x >> 5; i < TOK && t0 + i < p.T; i += blockDim.x >> 5) choose<L, DT>(p, t0 + i, hist, list + i * p.k);
   __syncthreads();
 }
 
@@ -146,26 +145,26 @@ __device__ __forceinline__ void place_chunk(const RouteParams& p, int64_t t0, in
 }
 
 // T <= TOK: the whole routing in one block.
-template <int L>
+template <int L, int DT>
 __global__ void __launch_bounds__(1024) route_small_kernel(const RouteParams p) {
   extern __shared__ int sm[];                        // next [2 E], list [TOK k]
   pdl_launch_dependents();
   pdl_wait();
   int* hist = sm + p.E;
   int* list = sm + 2 * p.E;
-  choose_chunk<L>(p, 0, hist, list);
+  choose_chunk<L, DT>(p, 0, hist, list);
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) sm[e] = 0;
   __syncthreads();
   place_chunk(p, 0, sm, list, true);
 }
 
 // One block per chunk of TOK tokens.
-template <int L>
+template <int L, int DT>
 __global__ void __launch_bounds__(1024) route_choose_kernel(const RouteParams p) {
   extern __shared__ int sm[];                        // hist [E], list [TOK k]
   pdl_launch_dependents();
   pdl_wait();
-  choose_chunk<L>(p, static_cast<int64_t>(blockIdx.x) * TOK, sm, sm + p.E);
+  choose_chunk<L, DT>(p, static_cast<int64_t>(blockIdx.x) * TOK, sm, sm + p.E);
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.E + e] = sm[e];
 }
 
@@ -318,20 +317,25 @@ int lb_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld
   if (r) return r;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) return launched(cudaMemsetAsync(offsets, 0, (E + 1) * sizeof(int), st), "moe_route");
-  moe::RouteParams p{logits, dtype, ldl, T, static_cast<int>(E), k, normalize ? 1 : 0, weights, experts, offsets, rows, slots,
+  moe::RouteParams p{logits, ldl, T, static_cast<int>(E), k, normalize ? 1 : 0, weights, experts, offsets, rows, slots,
                      static_cast<int*>(workspace)};
   const int g = static_cast<int>(chunks);
   const size_t sm = (2 * E + moe::TOK * k) * sizeof(int);
   cudaError_t e;
+#define LB_MOE_ROUTE_T(L, D)                                                                                          \
+  (g == 1 ? mx::launch_early(moe::route_small_kernel<L, D>, dim3(1), sm, st, p, 1024)                                 \
+          : mx::launch_early(moe::route_choose_kernel<L, D>, dim3(g), sm, st, p, 1024))
 #define LB_MOE_ROUTE(L)                                                                                               \
-  e = g == 1 ? mx::launch_early(moe::route_small_kernel<L>, dim3(1), sm, st, p, 1024)                                       \
-             : mx::launch_early(moe::route_choose_kernel<L>, dim3(g), sm, st, p, 1024)
+  e = dtype == LB_DT_F32    ? LB_MOE_ROUTE_T(L, LB_DT_F32)                                                            \
+      : dtype == LB_DT_BF16 ? LB_MOE_ROUTE_T(L, LB_DT_BF16)                                                           \
+                            : LB_MOE_ROUTE_T(L, LB_DT_F16)
   if (E <= 32) LB_MOE_ROUTE(1);
   else if (E <= 64) LB_MOE_ROUTE(2);
   else if (E <= 128) LB_MOE_ROUTE(4);
   else if (E <= 256) LB_MOE_ROUTE(8);
   else LB_MOE_ROUTE(32);
 #undef LB_MOE_ROUTE
+#undef LB_MOE_ROUTE_T
   if (e != cudaSuccess || g == 1) return launched(e, "moe_route");
   return launched(mx::launch_early(moe::route_place_kernel, dim3(g), sm, st, p, 1024), "moe_route");
 }
