@@ -8,6 +8,7 @@
 // since the divisors have at most 4 significant bits below 2 and the ties at most 5 (the nearest other quotient is more
 // than half an ulp away).  A block with a NaN or an infinity gets a NaN scale, so it stands for NaNs: nothing
 // is replaced in silence.  A zero block has scale byte 0.
+#include <type_traits>
 #include "lb_mx.cuh"
 #include "lb_kernels.h"
 
@@ -29,13 +30,41 @@ struct In<LB_DT_BF16> {
 template <>
 struct In<LB_DT_F16> : In<LB_DT_BF16> {};
 
+// Eight words from an address that is aligned to an element only (`off` bytes past p, which is 16-byte aligned; off is the same in
+// the whole warp): three aligned vectors, shifted.
+__device__ __forceinline__ void load8_off(const char* p, int off, uint32_t* w) {
+  uint32_t u[12];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint4 a = ldg_nc_v4(p + 16 * i);
+    u[4 * i] = a.x; u[4 * i + 1] = a.y; u[4 * i + 2] = a.z; u[4 * i + 3] = a.w;
+  }
+  const int sh = (off & 3) * 8;
+  auto take = [&](auto first) {
+    constexpr int F = decltype(first)::value;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __funnelshift_r(u[F + i], u[F + i + 1], sh);
+  };
+  switch (off >> 2) {
+    case 0: take(std::integral_constant<int, 0>()); break;
+    case 1: take(std::integral_constant<int, 1>()); break;
+    case 2: take(std::integral_constant<int, 2>()); break;
+    default: take(std::integral_constant<int, 3>()); break;
+  }
+}
+
 // 16 values of a row as they lie in memory (zeros past K); vec: rows are aligned to 32 bytes (2), 16 (1) or elements (0)
 template <int DT>
 struct Raw {
   static constexpr int NW = DT == LB_DT_F32 ? 16 : 8;
   uint32_t w[NW];
-  __device__ __forceinline__ void load(const char* p, int64_t left, int vec) {   // left: values of the row from p on
-    if (vec && left >= 16) {
+  // left: values of the row from p on; lo, hi: the tensor's first byte and the one past its last
+  __device__ __forceinline__ void load(const char* p, int64_t left, int vec, const char* lo, const char* hi) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    if (!vec && left >= 16 && p - off >= lo && p - off + (4 * NW + 16) <= hi) {
+#pragma unroll
+      for (int i = 0; i < NW / 8; ++i) load8_off(p - off + 32 * i, off, w + 8 * i);
+    } else if (vec && left >= 16) {
 #pragma unroll
       for (int i = 0; i < NW / 8; ++i) {
         if (vec == 2) {
@@ -110,19 +139,19 @@ __device__ __forceinline__ uint32_t codes8_any(const float* y, float s, float rs
   return e2m1_codes(up);
 }
 
-// Rows over the grid: a warp takes 512 values of a row (16 a thread).  wpr = 1, 2, 4 or 8 warps of a block lie side by side
-// along a row and blockIdx.y counts groups of eight; block x takes `per` rows one after another, so nothing of the column is worked
-// out twice and a group is looked up where it ends.
+// Rows over the grid: a warp takes 512 values of a row (16 a thread).  wpr warps of a block lie side by side along a row and
+// blockIdx.y counts groups of them; block x takes `per` rows one after another, so nothing of the column is worked out twice and a
+// group is looked up where it ends.
 struct Rows {
-  int wpr_log, per;
-  __device__ __forceinline__ int first() const { return static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x >> (5 + wpr_log)); }
+  int wpr, per;
+  __device__ __forceinline__ int first() const { return static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x >> 5) / wpr; }
   __device__ __forceinline__ int end(int64_t R) const {
     const int64_t e = (static_cast<int64_t>(blockIdx.x) + 1) * per;
     return static_cast<int>(e < R ? e : R);
   }
-  __device__ __forceinline__ int step() const { return 8 >> wpr_log; }
+  __device__ __forceinline__ int step() const { return static_cast<int>(blockDim.x >> 5) / wpr; }
   __device__ __forceinline__ int64_t col() const {
-    return (static_cast<int64_t>(blockIdx.y) * 8 + ((threadIdx.x >> 5) & ((1 << wpr_log) - 1))) * 512 + (threadIdx.x & 31) * 16;
+    return (static_cast<int64_t>(blockIdx.y) * wpr + static_cast<int>(threadIdx.x >> 5) % wpr) * 512 + (threadIdx.x & 31) * 16;
   }
 };
 
@@ -224,11 +253,12 @@ __global__ void __launch_bounds__(256, QUANT_BLOCKS) quant_kernel(const QuantPar
   if (r >= end) return;
   const char* const xc = static_cast<const char*>(p.x) + c0 * In<DT>::SIZE;
   const int64_t xrow = p.ldx * In<DT>::SIZE, left = p.K - c0;
+  const char* const x_end = static_cast<const char*>(p.x) + ((p.Rin - 1) * p.ldx + p.K) * In<DT>::SIZE;
   auto source = [&](int i) { return p.rows && i < end ? p.rows[i] : i; };
   auto load = [&](int src) {
     Raw<DT> x;
     if (src >= 0 && src < p.Rin) {
-      x.load(xc + src * xrow, left, p.vec);
+      x.load(xc + src * xrow, left, p.vec, static_cast<const char*>(p.x), x_end);
     } else {                                                     // no such row: zeros, and the error word says so
       if (lane == 0) atomicOr(&g_dev_errors, LB_DEVERR_BAD_INDEX);
       x.zero();
@@ -300,12 +330,13 @@ __global__ void __launch_bounds__(256) amax_kernel(const QuantParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t c0 = p.over.col();
   const char* const xc = static_cast<const char*>(p.x) + c0 * In<DT>::SIZE;
+  const char* const x_end = static_cast<const char*>(p.x) + ((p.Rin - 1) * p.ldx + p.K) * In<DT>::SIZE;
   const int step = p.over.step(), end = p.over.end(p.Rin);
   uint32_t am = 0;
 #pragma unroll 4
   for (int r = p.over.first(); r < end; r += step) {
     Raw<DT> x;
-    x.load(xc + r * (p.ldx * In<DT>::SIZE), p.K - c0, p.vec);
+    x.load(xc + r * (p.ldx * In<DT>::SIZE), p.K - c0, p.vec, static_cast<const char*>(p.x), x_end);
     const uint32_t m = x.amax();
     if (m < 0x7F800000u) {
       am = max(am, m);
@@ -321,8 +352,7 @@ __global__ void __launch_bounds__(256) amax_kernel(const QuantParams p) {
   if (lane == 0) red[threadIdx.x >> 5] = am;
   __syncthreads();
   if (threadIdx.x == 0) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) am = red[i] > am ? red[i] : am;
+    for (int i = 1; i < static_cast<int>(blockDim.x >> 5); ++i) am = red[i] > am ? red[i] : am;
     const_cast<float*>(p.part)[blockIdx.y * gridDim.x + blockIdx.x] = __uint_as_float(am);
   }
 }
@@ -353,16 +383,20 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
   const int gblocks = p.g.per > 0 ? static_cast<int>((p.g.per + 127) / 128) : 0;
   const int step = p.over.step(), end = p.over.end(p.R);
   constexpr int NW = ODT == LB_DT_F32 ? 16 : 8, ES = ODT == LB_DT_F32 ? 4 : 2;
-  if (c0 >= p.K) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t cw = c0 - lane * 16;           // the warp's first column
+  __shared__ uint32_t turn[8][32 * NW];
+  if (cw >= p.K) return;
   Walk walk(p.scales, c, acols, p.g);
   struct Packed { uint2 q; uint32_t s; bool in; };
   auto load = [&](int r) {                     // codes and scale byte of a row
     Packed u{make_uint2(0u, 0u), 0u, false};
     if (r < end) {
-      if (const uint8_t* sp = walk.at(p.g, off, base, gblocks, r)) {
+      const uint8_t* sp = walk.at(p.g, off, base, gblocks, r);
+      u.in = sp != nullptr;                    // the same in the whole warp
+      if (sp && c0 < p.K) {
         u.q = *reinterpret_cast<const uint2*>(p.codes + r * rb + c0 / 2);
         u.s = *sp;
-        u.in = true;
       }
     }
     return u;
@@ -413,23 +447,44 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
       }
     }
     char* o = static_cast<char*>(p.out) + (r * p.ldo + c0) * ES;
-    if (whole) {
+    if (p.vec) {
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < NW / 8; ++i) {
-        if (p.vec == 2) {
-          stg_v8(o + 32 * i, u + 8 * i);
-        } else {
-          reinterpret_cast<uint4*>(o)[2 * i] = make_uint4(u[8 * i], u[8 * i + 1], u[8 * i + 2], u[8 * i + 3]);
-          reinterpret_cast<uint4*>(o)[2 * i + 1] = make_uint4(u[8 * i + 4], u[8 * i + 5], u[8 * i + 6], u[8 * i + 7]);
+        for (int i = 0; i < NW / 8; ++i) {
+          if (p.vec == 2) {
+            stg_v8(o + 32 * i, u + 8 * i);
+          } else {
+            reinterpret_cast<uint4*>(o)[2 * i] = make_uint4(u[8 * i], u[8 * i + 1], u[8 * i + 2], u[8 * i + 3]);
+            reinterpret_cast<uint4*>(o)[2 * i + 1] = make_uint4(u[8 * i + 4], u[8 * i + 5], u[8 * i + 6], u[8 * i + 7]);
+          }
+        }
+      } else if (c0 < p.K) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (c0 + i >= p.K) continue;
+          if constexpr (ODT == LB_DT_F32) reinterpret_cast<uint32_t*>(o)[i] = u[i];
+          else reinterpret_cast<uint16_t*>(o)[i] = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
         }
       }
-    } else {
+    } else {                                   // odd rows: turned in shared memory so that a warp stores neighbours
+      uint32_t* tile = turn[threadIdx.x >> 5];
+#pragma unroll
+      for (int i = 0; i < NW; ++i) tile[lane * NW + ((i + lane) & (NW - 1))] = u[i];
+      __syncwarp();
+      const int n = static_cast<int>(p.K - cw < 512 ? p.K - cw : 512);
+      char* ow = static_cast<char*>(p.out) + (r * p.ldo + cw) * ES;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if (c0 + i >= p.K) continue;
-        if constexpr (ODT == LB_DT_F32) reinterpret_cast<uint32_t*>(o)[i] = u[i];
-        else reinterpret_cast<uint16_t*>(o)[i] = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
+        const int j = 32 * i + lane, l = j >> 4;               // value j of the warp's 512 is with lane l
+        if (j >= n) break;
+        if constexpr (ODT == LB_DT_F32) {
+          reinterpret_cast<uint32_t*>(ow)[j] = tile[l * NW + (((j & 15) + l) & (NW - 1))];
+        } else {
+          const uint32_t w = tile[l * NW + ((((j & 15) >> 1) + l) & (NW - 1))];
+          reinterpret_cast<uint16_t*>(ow)[j] = static_cast<uint16_t>(w >> (16 * (j & 1)));
+        }
       }
+      __syncwarp();
     }
   }
 }
@@ -456,11 +511,14 @@ __global__ void __launch_bounds__(256) scales_kernel(uint8_t* __restrict__ plain
 }
 
 constexpr int MAX_PARTS = LB_MX_PARTIALS;
-// At most `most` blocks over R rows of K values
-static dim3 over_rows(int64_t R, int64_t K, int64_t most, Rows* over) {
-  const int64_t segs = (K + 511) / 512;
-  over->wpr_log = segs > 4 ? 3 : (segs > 2 ? 2 : (segs > 1 ? 1 : 0));
-  const int64_t gy = (segs + 7) / 8, rpb = 8 >> over->wpr_log;
+// At most `most` blocks of up to eight warps over R rows of K values: long rows are cut evenly over as few groups of warps
+// as hold them, short ones share a block.
+static dim3 over_rows(int64_t R, int64_t K, int64_t most, Rows* over, int* threads) {
+  const int64_t segs = (K + 511) / 512, gy = (segs + 7) / 8;
+  over->wpr = static_cast<int>(segs > 4 ? (segs + gy - 1) / gy : (segs == 3 ? 4 : segs));
+  const int warps = segs > 4 ? over->wpr : 8;
+  *threads = warps * 32;
+  const int64_t rpb = warps / over->wpr;
   int64_t gx = (R + rpb - 1) / rpb;
   if (gx > most / gy) gx = most / gy;
   if (gx < 1) gx = 1;
@@ -549,24 +607,25 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
   p.codes = codes; p.scales = scales;
   p.vec = mx::row_vec(x, ldx, es);
   cudaError_t e;
+  int threads;
   if (fmt == LB_FMT_NVFP4 && !tensor_scale) {
     const int64_t segs = (K + 511) / 512;
     if (segs > 8 * mx::MAX_PARTS) return fail(LB_E_UNSUPPORTED, "lb_mx_quant: K above %d needs tensor_scale", 8 * 512 * mx::MAX_PARTS);
-    const dim3 nb = mx::over_rows(Rin > 0 ? Rin : 1, K, mx::MAX_PARTS, &p.over);
+    const dim3 nb = mx::over_rows(Rin > 0 ? Rin : 1, K, mx::MAX_PARTS, &p.over, &threads);
     p.part = auto_scale + 1;
     p.t_out = auto_scale;
     p.nparts = static_cast<int>(nb.x * nb.y);
-    e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::amax_kernel<LB_DT_F32>, nb, 0, st, p)
-        : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::amax_kernel<LB_DT_BF16>, nb, 0, st, p)
-                                : mx::launch_early(mx::amax_kernel<LB_DT_F16>, nb, 0, st, p);
+    e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::amax_kernel<LB_DT_F32>, nb, 0, st, p, threads)
+        : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::amax_kernel<LB_DT_BF16>, nb, 0, st, p, threads)
+                                : mx::launch_early(mx::amax_kernel<LB_DT_F16>, nb, 0, st, p, threads);
     if (e != cudaSuccess) return launched(e, "mx_amax");
   }
-  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::QUANT_BLOCKS, &p.over);
+  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::QUANT_BLOCKS, &p.over, &threads);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
 #define LB_MX_QUANT(F)                                                                                              \
-  e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::quant_kernel<F, LB_DT_F32>, blocks, sm, st, p)                 \
-      : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::quant_kernel<F, LB_DT_BF16>, blocks, sm, st, p)                \
-                              : mx::launch_early(mx::quant_kernel<F, LB_DT_F16>, blocks, sm, st, p)
+  e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::quant_kernel<F, LB_DT_F32>, blocks, sm, st, p, threads)                 \
+      : x_dtype == LB_DT_BF16 ? mx::launch_early(mx::quant_kernel<F, LB_DT_BF16>, blocks, sm, st, p, threads)                \
+                              : mx::launch_early(mx::quant_kernel<F, LB_DT_F16>, blocks, sm, st, p, threads)
   if (fmt == LB_FMT_MXFP4) LB_MX_QUANT(LB_FMT_MXFP4);
   else LB_MX_QUANT(LB_FMT_NVFP4);
 #undef LB_MX_QUANT
@@ -589,15 +648,16 @@ int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const fl
   DevInfo* d;
   if ((r = current(&d))) return r;
   mx::DequantParams p{codes, scales, tensor_scale, R, K, ldo, {offsets, static_cast<int>(G), per}, out,
-                      mx::row_vec(out, ldo, es), {0, 0}};
-  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::DEQUANT_BLOCKS, &p.over);
+                      mx::row_vec(out, ldo, es), {1, 0}};
+  int threads;
+  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::DEQUANT_BLOCKS, &p.over, &threads);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
 #define LB_MX_DEQUANT(F)                                                                                            \
-  e = out_dtype == LB_DT_F32    ? mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_F32>, blocks, sm, st, p)           \
-      : out_dtype == LB_DT_BF16 ? mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_BF16>, blocks, sm, st, p)          \
-                                : mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_F16>, blocks, sm, st, p)
+  e = out_dtype == LB_DT_F32    ? mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_F32>, blocks, sm, st, p, threads)           \
+      : out_dtype == LB_DT_BF16 ? mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_BF16>, blocks, sm, st, p, threads)          \
+                                : mx::launch_early(mx::dequant_kernel_mx<F, LB_DT_F16>, blocks, sm, st, p, threads)
   if (fmt == LB_FMT_MXFP4) LB_MX_DEQUANT(LB_FMT_MXFP4);
   else LB_MX_DEQUANT(LB_FMT_NVFP4);
 #undef LB_MX_DEQUANT

@@ -20,7 +20,7 @@
 // takes it into registers at once and converts and stores while the next tile's products run.
 //
 // Few units (decode, small layers): a cluster of S CTAs splits K; each leaves its float32 tile in its own shared
-// memory and every CTA adds its share of the columns over the cluster in rank order: one launch, no workspace, the
+// memory and every CTA adds its share of the outputs over the cluster in rank order: one launch, no workspace, the
 // same bits every time.
 //
 // All mbarrier waits are bounded (lb::mbar_wait); a timeout sets the device error word and the CTA drains.
@@ -58,20 +58,20 @@ struct Cfg {
   static constexpr int SFA = AT * 512, SFB = NB * AT * 512;
   static constexpr int B_BYTES = BT / CG * 128;                  // a pair's CTAs hold half of B each
   static constexpr int STAGE = A_BYTES + B_BYTES + SFA + SFB;
-  static constexpr int STAGES = BT == 256 ? (CG == 2 ? (FMT == LB_FMT_MXFP4 ? 6 : 5) : 4)
-                                          : (BT == 128 ? 6 : (FMT == LB_FMT_MXFP4 ? 8 : 7));
+  static constexpr int STAGES = BT == 256 ? (CG == 2 ? 5 : 4) : (BT == 128 ? (SWAP ? 5 : 6) : (FMT == LB_FMT_MXFP4 ? 8 : 7));
   static constexpr int ACCS = BT == 256 ? 1 : 2;
   static constexpr int SF_COLS = AT * 4 * (1 + NB);              // tensor memory columns of a stage's scales
   static_assert(ACCS * BT + STAGES * SF_COLS <= 512, "tensor memory");
-  static constexpr int PITCH = 129;                              // floats of a column in the cluster's tile
-  static_assert(CG == 2 || STAGES * STAGE >= BT * PITCH * 4, "the cluster's tile reuses the stages");
+  static constexpr int PITCH = 132;                              // floats of a token's row in the cluster's tile (128 outputs)
+  static_assert(BT == 256 || STAGES * STAGE >= 128 * PITCH * 4, "the cluster's tile reuses the stages");
   static constexpr int EW = SWAP ? 8 : 4;                        // epilogue warps
+  static constexpr int TURN = SWAP ? EW * 2048 : 0;              // 32 x 32 bf16 of each, for rows of y that are not aligned
   static constexpr int THREADS = (8 + EW) * 32;
   static constexpr int COLS = BT / (EW / 4);                     // columns of an epilogue warp
   static constexpr int TT = SWAP ? 128 * CG : BT, WT = SWAP ? BT : 128;   // tokens and weight rows of a unit
   static constexpr int LISTS = TT == 128 ? 2 : 3;                // words per group: off, base, (token tiles)
-  static int smem(int G) { return 1024 + STAGES * STAGE + 256 + (G ? LISTS * (G + 1) * 4 : 0); }
-  static_assert(1024 + STAGES * STAGE + 256 + LISTS * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
+  static int smem(int G) { return 1024 + STAGES * STAGE + TURN + 256 + (G ? LISTS * (G + 1) * 4 : 0); }
+  static_assert(1024 + STAGES * STAGE + TURN + 256 + LISTS * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
 };
 
 template <int FMT, int CG>
@@ -166,10 +166,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
-  float v;
-  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-               : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+               "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank));
   return v;
 }
 
@@ -264,7 +265,8 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
   uint8_t* bs = as + STAGES * A_BYTES;                           // STAGES x B_BYTES
   uint8_t* sfa = bs + STAGES * C::B_BYTES;
   uint8_t* sfb = sfa + STAGES * C::SFA;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sfb + STAGES * C::SFB);
+  uint8_t* turn = sfb + STAGES * C::SFB;
+  uint64_t* full = reinterpret_cast<uint64_t*>(turn + C::TURN);
   uint64_t* empty = full + STAGES;
   uint64_t* sf_full = empty + STAGES;                            // a stage's scales are in tensor memory
   uint64_t* acc_full = sf_full + STAGES;                         // [ACCS]
@@ -439,9 +441,19 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
           uint32_t v[16];
           tmem_ld_x16(d + c0, v);
           tc_wait_ld();
+          if (k1 <= k0) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            part[(h * HALF + c0 + j) * C::PITCH + rloc] = k1 > k0 ? __uint_as_float(v[j]) : 0.f;
+            for (int j = 0; j < 16; ++j) v[j] = 0u;
+          }
+          const int c = h * HALF + c0;
+          if (SWAP) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<uint4*>(part + rloc * C::PITCH + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) part[(c + j) * C::PITCH + rloc] = __uint_as_float(v[j]);
+          }
         }
       } else if (!SWAP) {
         const int64_t n = t.n0 + rloc;
@@ -506,14 +518,14 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
           }
           pack(g);
         }
-        if (ok) {
-          if ((p.vec & VEC_Y32) && cl >= HALF) {                 // whole 32-byte sectors
+        if (p.vec & VEC_Y16) {
+          if (ok && (p.vec & VEC_Y32) && cl >= HALF) {           // whole 32-byte sectors
 #pragma unroll
             for (int i = 0; i < HALF / 16; ++i) stg_v8(yr + 16 * i, o + 8 * i);
-          } else {
+          } else if (ok) {
 #pragma unroll
             for (int c0 = 0; c0 < HALF; c0 += 8) {
-              if ((p.vec & VEC_Y16) && c0 + 8 <= cl) {
+              if (c0 + 8 <= cl) {
                 *reinterpret_cast<uint4*>(yr + c0) = make_uint4(o[c0 / 2], o[c0 / 2 + 1], o[c0 / 2 + 2], o[c0 / 2 + 3]);
               } else {
 #pragma unroll
@@ -522,30 +534,58 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
               }
             }
           }
+        } else {
+          // rows that are not aligned: 32 x 32 values at a time turned in shared memory, so that a warp stores neighbours of one
+          // row (a lane storing its own row two bytes at a time took 82 us for [1082, 4178], 46 times its bytes' time)
+          const uint32_t mine = smem_u32(turn) + (warp - 8) * 2048;
+          const int rows = t.tn - half * 128 - q * 32;           // rows of this warp that exist
+          uint16_t* yw = p.y + (m - lane) * p.ldy + t.n0 + h * HALF;
+#pragma unroll
+          for (int c0 = 0; c0 < HALF; c0 += 32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)),
+                           "r"(o[c0 / 2 + 4 * i]), "r"(o[c0 / 2 + 4 * i + 1]), "r"(o[c0 / 2 + 4 * i + 2]), "r"(o[c0 / 2 + 4 * i + 3])
+                           : "memory");
+            __syncwarp();
+            if (c0 + lane < cl) {
+#pragma unroll 8
+              for (int r = 0; r < 32 && r < rows; ++r)
+                yw[r * p.ldy + c0 + lane] = static_cast<uint16_t>(
+                    lds_u16(mine + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2));
+            }
+            __syncwarp();
+          }
         }
       }
     }
   }
 
   if (S > 1) {
-    // every CTA adds its share of the columns over the cluster, in rank order
+    // every CTA adds its share of the outputs over the cluster in rank order, four neighbours of a row of y a thread
     __syncwarp();
     cluster_sync_all();
     if (u0 < units) {
       const Tile t = tile_at<C::TT, C::WT>(p, u0, off, base, tiles);
       const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
-      const int cols = SWAP ? t.nn : t.tn, lanes = SWAP ? t.tn : t.nn;
-      const int per = (cols + S - 1) / S, c0 = rank * per, c1 = c0 + per < cols ? c0 + per : cols;
-      const int w = c1 - c0;
-      for (int i = threadIdx.x; i < w * 128; i += C::THREADS) {
-        // consecutive threads take consecutive outputs of a row of y
-        const int c = c0 + (SWAP ? i % w : i >> 7), r = SWAP ? i / w : i & 127;
-        if (r >= lanes) continue;
-        const uint32_t a = smem_u32(smem) + (c * C::PITCH + r) * 4;
-        float v = ld_cluster_f32(a, 0);
-        for (int j = 1; j < S; ++j) v += ld_cluster_f32(a, j);
-        const int64_t m = t.tok0 + (SWAP ? r : c), n = t.n0 + (SWAP ? c : r);
-        store_one(p, m, n, v * alpha + bias_at(p, t.e * p.N + n));
+      const int per = (t.tn * 32 + S - 1) / S, i1 = (rank + 1) * per < t.tn * 32 ? (rank + 1) * per : t.tn * 32;
+      for (int i = rank * per + threadIdx.x; i < i1; i += C::THREADS) {
+        const int r = i >> 5, c = (i & 31) * 4;
+        if (c >= t.nn) continue;
+        const uint32_t a = smem_u32(smem) + (r * C::PITCH + c) * 4;
+        float4 u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < S) u[j] = ld_cluster_f32x4(a, j);
+        float v[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+        for (int j = 1; j < 8; ++j) {
+          if (j >= S) break;
+          v[0] += u[j].x; v[1] += u[j].y; v[2] += u[j].z; v[3] += u[j].w;
+        }
+        const int64_t m = t.tok0 + r, n = t.n0 + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < t.nn) store_one(p, m, n + j, v[j] * alpha + bias_at(p, t.e * p.N + n + j));
       }
     }
     cluster_sync_all();                     // no CTA leaves while its tile may be read
