@@ -511,8 +511,8 @@ __global__ void __launch_bounds__(256) scales_kernel(uint8_t* __restrict__ plain
 }
 
 constexpr int MAX_PARTS = LB_MX_PARTIALS;
-// At most `most` blocks of up to eight warps over R rows of K values: long rows are cut evenly over as few groups of warps
-// as hold them, short ones share a block.
+// At most `most` warps, in blocks of up to eight, over R rows of K values: long rows are cut evenly over as few groups of
+// warps as hold them, short ones share a block.
 static dim3 over_rows(int64_t R, int64_t K, int64_t most, Rows* over, int* threads) {
   const int64_t segs = (K + 511) / 512, gy = (segs + 7) / 8;
   over->wpr = static_cast<int>(segs > 4 ? (segs + gy - 1) / gy : (segs == 3 ? 4 : segs));
@@ -520,7 +520,7 @@ static dim3 over_rows(int64_t R, int64_t K, int64_t most, Rows* over, int* threa
   *threads = warps * 32;
   const int64_t rpb = warps / over->wpr;
   int64_t gx = (R + rpb - 1) / rpb;
-  if (gx > most / gy) gx = most / gy;
+  if (gx > most / (warps * gy)) gx = most / (warps * gy);
   if (gx < 1) gx = 1;
   over->per = static_cast<int>(((R + gx - 1) / gx + rpb - 1) / rpb * rpb);
   gx = (R + over->per - 1) / over->per;
@@ -611,7 +611,8 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
   if (fmt == LB_FMT_NVFP4 && !tensor_scale) {
     const int64_t segs = (K + 511) / 512;
     if (segs > 8 * mx::MAX_PARTS) return fail(LB_E_UNSUPPORTED, "lb_mx_quant: K above %d needs tensor_scale", 8 * 512 * mx::MAX_PARTS);
-    const dim3 nb = mx::over_rows(Rin > 0 ? Rin : 1, K, mx::MAX_PARTS, &p.over, &threads);
+    // at least five warps a block, so at most MAX_PARTS blocks
+    const dim3 nb = mx::over_rows(Rin > 0 ? Rin : 1, K, 5 * mx::MAX_PARTS, &p.over, &threads);
     p.part = auto_scale + 1;
     p.t_out = auto_scale;
     p.nparts = static_cast<int>(nb.x * nb.y);
@@ -620,7 +621,7 @@ int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int
                                 : mx::launch_early(mx::amax_kernel<LB_DT_F16>, nb, 0, st, p, threads);
     if (e != cudaSuccess) return launched(e, "mx_amax");
   }
-  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::QUANT_BLOCKS, &p.over, &threads);
+  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::QUANT_BLOCKS * 8, &p.over, &threads);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
 #define LB_MX_QUANT(F)                                                                                              \
   e = x_dtype == LB_DT_F32    ? mx::launch_early(mx::quant_kernel<F, LB_DT_F32>, blocks, sm, st, p, threads)                 \
@@ -650,7 +651,7 @@ int lb_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, const fl
   mx::DequantParams p{codes, scales, tensor_scale, R, K, ldo, {offsets, static_cast<int>(G), per}, out,
                       mx::row_vec(out, ldo, es), {1, 0}};
   int threads;
-  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::DEQUANT_BLOCKS, &p.over, &threads);
+  const dim3 blocks = mx::over_rows(R, K, static_cast<int64_t>(d->sms) * mx::DEQUANT_BLOCKS * 8, &p.over, &threads);
   const size_t sm = G > 0 && per == 0 ? 2 * (G + 1) * sizeof(int) : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
