@@ -17,7 +17,10 @@ GEMM above; the residual adds are the kernels' accumulate epilogue.  The normali
 gate/up, head) go through ``kernels.linear_rms``: for decode the RMSNorm runs inside the GEMV's activation
 staging, for prefill ``lb_rmsnorm`` precedes the GEMM (the same bits either way).  The QKV split with rotary
 embedding and the cache write (``lb_qkv_prep``) and the SwiGLU product (``lb_act_mul``) are the library's
-kernels too.  Embedding lookup and attention over the KV cache are torch operations (attention is not
+kernels too.  With ``fmt`` "mxfp4" or "nvfp4" every projection is a product of microscaled 4-bit operands
+(``microscale.linear``): the weights are packed once and the activations (after the RMSNorm where there is one) are
+quantised to the same format on the way in; ``E`` experts then may take the place of the dense MLP
+(``experts.ExpertMLP``: router, ``topk`` experts of a token, products by expert).  Embedding lookup and attention over the KV cache are torch operations (attention is not
 on the quantized-linear path this library rebuilds).  Activations are bf16; the KV cache is bf16.
 
 Weights are random (seeded, N(0, 0.02) projections, unit norms), as configs[3] specifies; there is no
@@ -31,8 +34,9 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import kernels as Kn
-from ._lib import FMT_INT4_G128, FMT_INT8_ROW, FMT_FP8_E4M3, FMT_FP4_E2M1, LowbitError, LB_E_ARG
+from . import experts, kernels as Kn, microscale
+from ._lib import (FMT_INT4_G128, FMT_INT8_ROW, FMT_FP8_E4M3, FMT_FP4_E2M1, FMT_MXFP4, FMT_NVFP4, MICROSCALED_FMT, LowbitError,
+                   LB_E_ARG)
 
 __all__ = ["DecoderConfig", "QuantDecoder", "KVCache"]
 
@@ -50,6 +54,8 @@ class DecoderConfig:
     eps: float = 1e-5
     theta: float = 10000.0
     wstd: float = 0.02
+    E: int = 0             # experts in the place of each layer's MLP (0: dense; microscaled formats only)
+    topk: int = 2          # experts of a token
 
 
 class KVCache:
@@ -89,10 +95,35 @@ class _Proj:
         return Kn.dequant_minifloat(self.fmt, self.codes, self.N, self.K, self.scales)
 
 
+class _MxProj:
+    """One microscaled projection: an ``MxTensor`` [N, K] times activations quantised on the way in."""
+    __slots__ = ("w",)
+
+    def __init__(self, W, fmt):
+        self.w = microscale.quantize(W, fmt)
+
+    def __call__(self, x, out=None, accumulate=False, static=False, ln=None, eps=1e-6):
+        if ln is not None:
+            x = Kn.rmsnorm(x, ln, eps=eps)
+        return microscale.linear(x, self.w, out=out, accumulate=accumulate)
+
+    @property
+    def codes(self):
+        return self.w.codes
+
+    @property
+    def scales(self):
+        return self.w.scales
+
+    def dequantized(self):
+        return self.w.dequantize()
+
+
 class QuantDecoder:
     """The decoder of configs[3] with packed low-bit projections (see the module docstring)."""
 
-    _FMTS = {"int4": FMT_INT4_G128, "int8": FMT_INT8_ROW, "fp8_e4m3": FMT_FP8_E4M3, "fp4_e2m1": FMT_FP4_E2M1}
+    _FMTS = {"int4": FMT_INT4_G128, "int8": FMT_INT8_ROW, "fp8_e4m3": FMT_FP8_E4M3, "fp4_e2m1": FMT_FP4_E2M1,
+             "mxfp4": FMT_MXFP4, "nvfp4": FMT_NVFP4}
 
     def __init__(self, cfg=None, device="cuda", fmt="int4", seed=0, max_positions=8192):
         self._setup(cfg or DecoderConfig(), device, fmt, max_positions)
@@ -103,9 +134,15 @@ class QuantDecoder:
 
         def proj(n, k):
             W = torch.randn((n, k), generator=g, device=self.dev) * cfg.wstd
-            p = _Proj(W, self.fmt)
+            p = self._proj(W)
             del W
             return p
+
+        def expert_mlp():
+            def randn(*shape):
+                return torch.randn(shape, generator=g, device=self.dev) * cfg.wstd
+            return experts.ExpertMLP(randn(cfg.E, cfg.H), randn(cfg.E, 2 * cfg.I, cfg.H), randn(cfg.E, cfg.H, cfg.I), cfg.topk,
+                                     self.fmt_name)
 
         self.embed = (torch.randn((cfg.V, cfg.H), generator=g, device=self.dev) * cfg.wstd * 50).to(torch.bfloat16)
         self.layers = []
@@ -115,8 +152,7 @@ class QuantDecoder:
                 "qkv": proj(width, cfg.H),
                 "o": proj(cfg.H, cfg.nh * cfg.dh),
                 "ln2": torch.ones(cfg.H, dtype=torch.bfloat16, device=self.dev),
-                "gu": proj(2 * cfg.I, cfg.H),
-                "down": proj(cfg.H, cfg.I),
+                **({"moe": expert_mlp()} if cfg.E else {"gu": proj(2 * cfg.I, cfg.H), "down": proj(cfg.H, cfg.I)}),
             })
         self.norm = torch.ones(cfg.H, dtype=torch.bfloat16, device=self.dev)
         self.head = proj(cfg.V, cfg.H)
@@ -126,7 +162,9 @@ class QuantDecoder:
         self.dev = torch.device(device)
         if fmt not in self._FMTS:
             raise LowbitError(LB_E_ARG, f"projection format '{fmt}' is not one of {sorted(self._FMTS)}")
-        self.fmt = self._FMTS[fmt]
+        self.fmt, self.fmt_name = self._FMTS[fmt], fmt
+        if cfg.E and fmt not in MICROSCALED_FMT:
+            raise LowbitError(LB_E_ARG, f"experts need a microscaled format {sorted(MICROSCALED_FMT)}, got '{fmt}'")
         half = cfg.dh // 2
         inv = 1.0 / (cfg.theta ** (torch.arange(half, device=self.dev, dtype=torch.float64) / half))
         self._inv = inv.float()                                        # rotary frequencies
@@ -134,6 +172,9 @@ class QuantDecoder:
         self._cos = torch.cos(ang).float().contiguous()                # [positions, dh / 2]
         self._sin = torch.sin(ang).float().contiguous()
         self.max_positions = max_positions
+
+    def _proj(self, W):
+        return _MxProj(W, self.fmt_name) if self.fmt_name in MICROSCALED_FMT else _Proj(W, self.fmt)
 
     @classmethod
     def from_weights(cls, hf_cfg, W, device="cuda", fmt="int4", max_positions=None):
@@ -167,7 +208,7 @@ class QuantDecoder:
                                    dtype=torch.float32).to(self.dev).contiguous()
 
         def proj(*names):
-            return _Proj(torch.cat([dev32(W[n]) for n in names], 0), self.fmt)
+            return self._proj(torch.cat([dev32(W[n]) for n in names], 0))
 
         def vec(n):
             return dev32(W[n]).to(torch.bfloat16)
@@ -192,7 +233,9 @@ class QuantDecoder:
     def weight_bytes(self):
         def nb(p):
             return p.codes.numel() * p.codes.element_size() + p.scales.numel() * p.scales.element_size()
-        return sum(nb(p) for Ld in self.layers for p in (Ld["qkv"], Ld["o"], Ld["gu"], Ld["down"])) + nb(self.head)
+        def mlp(Ld):
+            return (Ld["moe"].gate_up, Ld["moe"].down) if "moe" in Ld else (Ld["gu"], Ld["down"])
+        return sum(nb(p) for Ld in self.layers for p in (Ld["qkv"], Ld["o"], *mlp(Ld))) + nb(self.head)
 
     def new_cache(self, batch, cap):
         if cap > self.max_positions:
@@ -217,6 +260,9 @@ class QuantDecoder:
             attn = F.scaled_dot_product_attention(q, kc, vc, attn_mask=mask, enable_gqa=True)
         o_in = attn.transpose(1, 2).reshape(M, cfg.nh * cfg.dh).contiguous()
         Ld["o"](o_in, out=X, accumulate=True, static=static)
+        if "moe" in Ld:
+            Ld["moe"](Kn.rmsnorm(X, Ld["ln2"], eps=cfg.eps), out=X, accumulate=True)
+            return
         gu = Ld["gu"](X, static=static, ln=Ld["ln2"], eps=cfg.eps)
         m = Kn.act_mul(gu, cfg.I, 0)
         Ld["down"](m, out=X, accumulate=True, static=static)

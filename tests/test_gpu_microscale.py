@@ -354,3 +354,28 @@ def test_refusals(mx):
         with pytest.raises(LowbitError):
             f()
             pytest.fail(f"case {i} was taken")
+
+
+def test_offsets_past_32_bits(mx):
+    """More than 2^31 values: the last rows' codes, scales and values lie beyond 32-bit offsets."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    R, K = 40000, 57344
+    x = torch.empty((R, K), device="cuda", dtype=torch.bfloat16)
+    x[:8].normal_()
+    x[8:-8] = 1.0
+    x[-8:].normal_()
+    q = mx.quantize(x, "mxfp4")
+    ends = torch.cat((x[:8], x[-8:]))
+    want = ora.quantize(f64(ends), "mxfp4")[2]
+    v = q.dequantize(torch.bfloat16)
+    assert np.array_equal(f64(torch.cat((v[:8], v[-8:]))), want)
+    assert bool((v[8:-8] == 1).all())
+    del v
+    del x
+    # the same codes as a weight of 40000 rows, read at both ends
+    a = mx.quantize(torch.randn((3, K), device="cuda"), "mxfp4")
+    y = mx.linear(a, q)
+    ref = f64(a.dequantize().double()) @ want.T
+    mass = np.abs(f64(a.dequantize().double())) @ np.abs(want).T
+    assert_rounds(torch.cat((y[:, :8], y[:, -8:]), 1), ref, sum_error(mass, K))
