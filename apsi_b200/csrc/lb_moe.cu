@@ -292,7 +292,7 @@ extern "C" {
 int lb_moe_route_workspace_size(int64_t T, int64_t E, size_t* bytes) {
   if (!bytes) return fail(LB_E_ARG, "lb_moe_route_workspace_size: bytes is NULL");
   if (T < 0 || E <= 0) return fail(LB_E_ARG, "lb_moe_route_workspace_size: bad sizes");
-  *bytes = static_cast<size_t>((T + moe::TOK - 1) / moe::TOK) * E * sizeof(int);
+  *bytes = T <= moe::TOK ? 0 : static_cast<size_t>((T + moe::TOK - 1) / moe::TOK) * E * sizeof(int);
   return LB_OK;
 }
 
@@ -309,7 +309,7 @@ int lb_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld
       !aligned(rows, 4) || !aligned(slots, 4) || !aligned(workspace, 4))
     return fail(LB_E_ALIGN, "lb_moe_route: pointers must be element aligned");
   const int64_t chunks = (T + moe::TOK - 1) / moe::TOK;
-  const size_t need = static_cast<size_t>(chunks) * E * sizeof(int);
+  const size_t need = chunks > 1 ? static_cast<size_t>(chunks) * E * sizeof(int) : 0;
   if (need && (!workspace || ws_bytes < need))
     return fail(LB_E_WORKSPACE, "lb_moe_route: workspace of %zu bytes needed (got %zu)", need, workspace ? ws_bytes : 0);
   DevInfo* d;

@@ -38,16 +38,17 @@ def route(logits, k, normalize=True):
         raise LowbitError(LB_E_ARG, f"1 to {MX_MAX_GROUPS} experts and k of 1 to min(E, 32), got E = {E}, k = {k}")
     if E > 1 and logits.stride(1) != 1:
         raise LowbitError(LB_E_ARG, "the logits of a token must be next to each other")
-    n = T * k
+    n, count = T * k, (T + 63) // 64 * E if T > 64 else 0      # the workspace: a count per expert and 64 tokens
     weights = logits.new_empty((T, k), dtype=torch.float32)
-    # experts, slots, rows, offsets and the workspace (one count per expert and 64 tokens) in one allocation
-    ints = logits.new_empty(3 * n + E + 1 + (T + 63) // 64 * E, dtype=torch.int32)
-    experts, slots, rows, offsets, _ = ints.split((n, n, n, E + 1, ints.shape[0] - 3 * n - E - 1))
-    at = ints.data_ptr()
-    _launch(logits.get_device(), "lb_moe_route", logits.data_ptr(), dt, T, E, logits.stride(0) if T > 1 else E, k,
-            1 if normalize else 0, weights.data_ptr(), at, at + 12 * n, at + 8 * n, at + 4 * n, at + 12 * n + 4 * (E + 1),
-            4 * ((T + 63) // 64 * E))
-    return Route(weights, experts.view(T, k), offsets, rows, slots.view(T, k))
+    experts = logits.new_empty((T, k), dtype=torch.int32)
+    slots = torch.empty_like(experts)
+    rows = experts.new_empty(n)
+    offsets = experts.new_empty(E + 1 + count)
+    at = offsets.data_ptr()
+    _launch(logits.get_device(), "lb_moe_route", logits.data_ptr(), dt, T, E, logits.stride(0) if T > 1 else E, k, 1 if normalize else 0,
+            weights.data_ptr(), experts.data_ptr(), at, rows.data_ptr(), slots.data_ptr(), at + 4 * (E + 1) if count else None,
+            4 * count)
+    return Route(weights, experts, offsets[:E + 1] if count else offsets, rows, slots)
 
 
 def combine(z, weights, slots, out=None, accumulate=False):
@@ -58,12 +59,14 @@ def combine(z, weights, slots, out=None, accumulate=False):
     dev = z.get_device()
     if z.dtype != torch.bfloat16 or z.dim() != 2 or (z.shape[1] > 1 and z.stride(1) != 1):
         raise LowbitError(LB_E_ARG, "z must be bfloat16 [R, H] with unit column stride")
-    for t, dtype, name in ((weights, torch.float32, "weights"), (slots, torch.int32, "slots")):
-        if (not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype != dtype or t.dim() != 2 or not t.is_contiguous()
-                or t.shape != weights.shape or t.shape[1] == 0):
-            raise LowbitError(LB_E_ARG, f"{name} must be a contiguous {dtype} tensor [T, k] on {z.device}")
+    if (not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.dim() != 2 or weights.shape[1] == 0
+            or not weights.is_contiguous() or weights.get_device() != dev):
+        raise LowbitError(LB_E_ARG, f"weights must be a contiguous float32 tensor [T, k] on {z.device}")
+    if (not isinstance(slots, torch.Tensor) or slots.dtype != torch.int32 or slots.shape != weights.shape
+            or not slots.is_contiguous() or slots.get_device() != dev):
+        raise LowbitError(LB_E_ARG, f"slots must be a contiguous int32 tensor of weights' sizes on {z.device}")
     (T, k), (R, H) = weights.shape, z.shape
-    y, ld = _output(out, T, H, z, accumulate)
+    y, ld = (z.new_empty((T, H)), H) if out is None and not accumulate else _output(out, T, H, z, accumulate)
     _launch(dev, "lb_moe_combine", z.data_ptr(), R, z.stride(0) if R > 1 else H, weights.data_ptr(), slots.data_ptr(), T, k, H,
             1 if accumulate else 0, y.data_ptr(), ld)
     return y

@@ -304,7 +304,8 @@ int lb_mx_scales(int fmt, uint8_t* plain, int64_t ld, int64_t G, int64_t N, int6
                  void* stream);
 
 /* y[m, n] = x_t w_t sum_k x[m, k] w[n, k] over the values the codes stand for (+ bias[n], bf16) (+ y[m, n] if accumulate),
- * float32 accumulation, bf16 out with row stride ldy.  x [M, K] and w [N, K] in the same format, each one group. */
+ * float32 accumulation, bf16 out with row stride ldy.  x [M, K] and w [N, K] in the same format, each one group; x_t, w_t:
+ * device scalars, NULL: 1.  No workspace; the same bits every time.  Few output tiles: a cluster of CTAs splits K. */
 int lb_mx_linear(int fmt, const uint8_t* x_codes, const uint8_t* x_scales, const float* x_tscale, int64_t M, int64_t K,
                  const uint8_t* w_codes, const uint8_t* w_scales, const float* w_tscale, int64_t N, const void* bias,
                  int accumulate, void* y, int64_t ldy, void* stream);
@@ -324,7 +325,7 @@ int lb_mx_linear_grouped(int fmt, const uint8_t* x_codes, const uint8_t* x_scale
  * experts, divided by its sum over the chosen ones if normalize.  NaN counts as -inf, -inf weighs 0, a row of
  * nothing else weighs 0 throughout, +inf shares the weight evenly.  The T k pairs (t, j) sorted by expert, in order
  * within one: offsets [E + 1], rows [T k] (the token of each place), slots [T, k] (the place of each pair).  Workspace:
- * lb_moe_route_workspace_size bytes. */
+ * lb_moe_route_workspace_size bytes (none for T <= 64), contents need no initialisation. */
 int lb_moe_route_workspace_size(int64_t T, int64_t E, size_t* bytes);
 int lb_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, int k, int normalize, float* weights,
                  int* experts, int* offsets, int* rows, int* slots, void* workspace, size_t ws_bytes, void* stream);

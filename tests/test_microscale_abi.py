@@ -33,6 +33,7 @@ def test_sizes(lib):
     assert lib.lb_mx_scale_bytes(9, 3, 32, 0, 0) == -1 and lib.lb_mx_scale_bytes(MX, 3, 0, 0, 0) == -1
     n = ctypes.c_size_t(0)
     assert lib.lb_moe_route_workspace_size(65, 8, ctypes.byref(n)) == 0 and n.value == 2 * 8 * 4
+    assert lib.lb_moe_route_workspace_size(64, 8, ctypes.byref(n)) == 0 and n.value == 0
     from apsi_b200 import microscale
     for fmt, f in _lib.MICROSCALED_FMT.items():
         for R, K, G, per in ((0, 5, 0, 0), (1, 1, 0, 0), (300, 1000, 0, 0), (300, 1000, 7, 0), (3, 64, 7, 0), (12, 256, 4, 3)):
@@ -67,11 +68,11 @@ def test_refusals_before_a_device_is_touched(lib):
     assert grouped(G=0) == E and grouped(off=null) == E and grouped(G=1025) == E and grouped(N=9) == E
     assert grouped(off=ctypes.c_void_p((1 << 20) + 2)) == A
 
-    def route(dt=0, T=4, E_=8, ld=8, k=2, w=p, off=p, ws=p, n=1 << 10):
+    def route(dt=0, T=100, E_=8, ld=8, k=2, w=p, off=p, ws=p, n=1 << 10):
         return lib.lb_moe_route(p, dt, T, E_, ld, k, 1, w, p, off, p, p, ws, n, null)
     assert route(dt=4) == E and route(E_=0) == E and route(E_=1025, ld=1025) == E and route(ld=7) == E and route(k=0) == E
     assert route(k=9) == E and route(w=null) == E and route(off=null) == E and route(ws=null) == _lib.LB_E_WORKSPACE
-    assert route(n=31) == _lib.LB_E_WORKSPACE
+    assert route(n=63) == _lib.LB_E_WORKSPACE
 
     def combine(z=p, rows=8, ldz=16, w=p, s=p, T=4, k=2, H=16, y=p, ldy=16):
         return lib.lb_moe_combine(z, rows, ldz, w, s, T, k, H, 0, y, ldy, null)
