@@ -9,11 +9,13 @@
 // that read it are done (the stage's own `empty` barrier).  As tcgen05.cp they cost the tensor pipe about 45 cycles
 // an atom: with 12 atoms against 512 cycles of nvfp4 products a stage that was the bound.
 //
-//   SWAP = false   few tokens: A = 128 weight rows, B = BT (64 or 128) tokens; an output column is a token, a lane a weight row
-//   SWAP = true    many: A = 128 tokens, B = BT weight rows; a lane is a token and holds runs of columns
-//   CG = 2         a pair of CTAs (cta_group::2) on 256 tokens x 256 weight rows: each loads its own 128 tokens and half of
-//                  the weight rows, so a product needs 16 KB of codes from L2 for every 128 x 256 outputs and 64 K, not 24;
-//                  with 1-CTA tiles L2 -> SM traffic (12.5 TB/s measured) was the bound
+// A (the rows of the accumulator, tensor memory's lanes) is 128 weight rows, B (its columns) up to BT = 64, 128 or 256 tokens; a
+// tile with fewer tokens multiplies only those (rounded up to 16, a pair 32), so a ragged group's last tile costs what it holds.
+// Weights on the lanes also make a warp's store 32 neighbours of a row of y, whatever its alignment.
+//   BT = 256   a pair of CTAs (cta_group::2) on 256 weight rows x 256 tokens: each loads its own 128 weight rows and half of
+//              the tokens, so a product needs 16 KB of codes from L2 for every 128 x 256 outputs and 256 of K, not 24
+// What bounds a pair's stage is the shared memory: 35 KB (mxfp4) or 39 KB (nvfp4) written by TMA, 32 KB read by the products, 12 or
+// 24 KB by the four warps that take the scales, at 128 bytes a cycle 620 or 740 cycles against 512 of products.
 //
 // Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales, 8.. epilogue (4 or 8 warps; warp w reads lanes
 // 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
@@ -44,34 +46,32 @@ struct GemmMxParams {
   int acc;
   Groups g;                 // of the rows of x (ragged); G == 0: dense
   int ksteps, tiles_w, tiles_t;
-  int vec;                  // VEC_*
 };
-constexpr int VEC_Y16 = 1, VEC_Y32 = 2, VEC_BIAS = 4;   // rows of y 16 / 32-byte aligned, rows of bias 16-byte aligned
 
 constexpr int A_BYTES = 128 * 128;
 constexpr int SMEM_MAX = 227 * 1024;
 
-template <int FMT, int BT, bool SWAP, int CG>
+template <int FMT, int BT>
 struct Cfg {
+  static constexpr int CG = BT == 256 ? 2 : 1;                   // CTAs of a tile
+  static constexpr int WT = 128 * CG;                            // its weight rows
   static constexpr int AT = atoms256(FMT);                       // scale atoms of a row block per stage
-  static constexpr int NB = BT > 128 ? 2 : 1;                    // row blocks of the B tile
+  static constexpr int NB = BT > 128 ? 2 : 1;                    // row blocks of the tokens
   static constexpr int SFA = AT * 512, SFB = NB * AT * 512;
-  static constexpr int B_BYTES = BT / CG * 128;                  // a pair's CTAs hold half of B each
+  static constexpr int B_BYTES = BT / CG * 128;                  // a pair's CTAs hold half of the tokens each
   static constexpr int STAGE = A_BYTES + B_BYTES + SFA + SFB;
-  static constexpr int STAGES = BT == 256 ? (CG == 2 ? 5 : 4) : (BT == 128 ? (SWAP ? 5 : 6) : (FMT == LB_FMT_MXFP4 ? 8 : 7));
+  static constexpr int STAGES = BT == 64 ? (FMT == LB_FMT_MXFP4 ? 8 : 7) : (BT == 256 && FMT == LB_FMT_NVFP4 ? 5 : 6);
   static constexpr int ACCS = BT == 256 ? 1 : 2;
   static constexpr int SF_COLS = AT * 4 * (1 + NB);              // tensor memory columns of a stage's scales
   static_assert(ACCS * BT + STAGES * SF_COLS <= 512, "tensor memory");
   static constexpr int PITCH = 132;                              // floats of a token's row in the cluster's tile (128 outputs)
-  static_assert(BT == 256 || STAGES * STAGE >= 128 * PITCH * 4, "the cluster's tile reuses the stages");
-  static constexpr int EW = SWAP ? 8 : 4;                        // epilogue warps
-  static constexpr int TURN = SWAP ? EW * 2048 : 0;              // 32 x 32 bf16 of each, for rows of y that are not aligned
+  static_assert(CG == 2 || STAGES * STAGE >= BT * PITCH * 4, "the cluster's tile reuses the stages");
+  static constexpr int EW = 4 * CG;                              // epilogue warps
   static constexpr int THREADS = (8 + EW) * 32;
-  static constexpr int COLS = BT / (EW / 4);                     // columns of an epilogue warp
-  static constexpr int TT = SWAP ? 128 * CG : BT, WT = SWAP ? BT : 128;   // tokens and weight rows of a unit
-  static constexpr int LISTS = TT == 128 ? 2 : 3;                // words per group: off, base, (token tiles)
-  static int smem(int G) { return 1024 + STAGES * STAGE + TURN + 256 + (G ? LISTS * (G + 1) * 4 : 0); }
-  static_assert(1024 + STAGES * STAGE + TURN + 256 + LISTS * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
+  static constexpr int COLS = BT / CG;                           // columns of an epilogue warp
+  static constexpr int LISTS = BT == 128 ? 2 : 3;                // words per group: off, base, (token tiles)
+  static int smem(int G) { return 1024 + STAGES * STAGE + 256 + (G ? LISTS * (G + 1) * 4 : 0); }
+  static_assert(1024 + STAGES * STAGE + 256 + LISTS * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
 };
 
 template <int FMT, int CG>
@@ -189,7 +189,7 @@ __device__ __forceinline__ int total_units(const GemmMxParams& p, const int* til
 }
 
 // off, base: load_groups; tiles: token tiles before group e (tiles of 128: base itself)
-template <int TT, int WT>
+template <int BT, int WT>
 __device__ __forceinline__ Tile tile_at(const GemmMxParams& p, int u, const int* off, const int* base, const int* tiles) {
   int t, w, e = 0;
   int64_t r0 = 0, rows = p.M, blk0 = 0;
@@ -210,11 +210,11 @@ __device__ __forceinline__ Tile tile_at(const GemmMxParams& p, int u, const int*
   }
   Tile r;
   r.e = e;
-  r.tok0 = r0 + static_cast<int64_t>(t) * TT;
-  const int64_t left = rows - static_cast<int64_t>(t) * TT;
-  r.tn = static_cast<int>(left < TT ? left : TT);
-  r.tblk = blk0 + (static_cast<int64_t>(t) * TT >> 7);
-  r.toff = (t * TT) & 127;
+  r.tok0 = r0 + static_cast<int64_t>(t) * BT;
+  const int64_t left = rows - static_cast<int64_t>(t) * BT;
+  r.tn = static_cast<int>(left < BT ? left : BT);
+  r.tblk = blk0 + (static_cast<int64_t>(t) * BT >> 7);
+  r.toff = (t * BT) & 127;
   r.n0 = static_cast<int64_t>(w) * WT;
   r.nn = static_cast<int>(p.N - r.n0 < WT ? p.N - r.n0 : WT);
   r.wrow = static_cast<int64_t>(e) * p.N + r.n0;
@@ -231,42 +231,22 @@ __device__ __forceinline__ void store_one(const GemmMxParams& p, int64_t m, int6
   *yp = f32_to_bf16_bits_g(v);
 }
 
-// v[j] += row[j] (bf16) for the j < n that exist; vec: the row is 16-byte aligned
-__device__ __forceinline__ void add_row(uint32_t (&v)[32], const uint16_t* row, int n, bool vec) {
-  if (vec && n >= 32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + 8 * i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[8 * i + 2 * j] = __float_as_uint(__uint_as_float(v[8 * i + 2 * j]) + __uint_as_float(w[j] << 16));
-        v[8 * i + 2 * j + 1] = __float_as_uint(__uint_as_float(v[8 * i + 2 * j + 1]) + __uint_as_float(w[j] & 0xFFFF0000u));
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(static_cast<uint32_t>(row[j]) << 16));
-  }
-}
+constexpr int TOK_BOX = 16;                 // token rows of the smaller TMA box: a few tokens do not bring in others'
 
-constexpr int TOK_BOX = 16;                 // token rows of a TMA box (SWAP = false): only boxes with tokens are read
-
-template <int FMT, int BT, bool SWAP, int CG>
-__global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
-    mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const GemmMxParams p) {
-  using C = Cfg<FMT, BT, SWAP, CG>;
-  static_assert(CG == 1 || (SWAP && BT == 256), "pairs take 256 x 256 tiles");
-  constexpr int STAGES = C::STAGES, AT = C::AT;
+// tm_b, tm_bs: the tokens' codes in boxes of all of a CTA's rows, and of TOK_BOX
+template <int FMT, int BT>
+__global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                   const __grid_constant__ CUtensorMap tm_bs, const GemmMxParams p) {
+  using C = Cfg<FMT, BT>;
+  constexpr int STAGES = C::STAGES, AT = C::AT, CG = C::CG;
   extern __shared__ __align__(1024) uint8_t dyn_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* as = smem;                                            // STAGES x 16 KB
   uint8_t* bs = as + STAGES * A_BYTES;                           // STAGES x B_BYTES
   uint8_t* sfa = bs + STAGES * C::B_BYTES;
   uint8_t* sfb = sfa + STAGES * C::SFA;
-  uint8_t* turn = sfb + STAGES * C::SFB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(turn + C::TURN);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sfb + STAGES * C::SFB);
   uint64_t* empty = full + STAGES;
   uint64_t* sf_full = empty + STAGES;                            // a stage's scales are in tensor memory
   uint64_t* acc_full = sf_full + STAGES;                         // [ACCS]
@@ -293,6 +273,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
     fence_barrier_init();
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
+    prefetch_tmap(&tm_bs);
   }
   if (warp == 1) tmem_alloc_all<CG>(tmem_holder);
   pdl_wait();                                                    // what earlier kernels wrote is read from here on
@@ -302,7 +283,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
       int run = 0;
       for (int e0 = 0; e0 <= p.g.G; e0 += 32) {
         const int e = e0 + lane;
-        const int n = e < p.g.G ? (off[e + 1] - off[e] + C::TT - 1) / C::TT : 0;
+        const int n = e < p.g.G ? (off[e + 1] - off[e] + BT - 1) / BT : 0;
         int s = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -335,22 +316,23 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
     if (elect_one()) {
       uint32_t it = 0;
       for (int u = u0; u < units; u += du) {
-        const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
-        const int64_t arow = SWAP ? t.tok0 + half * 128 : t.wrow, brow = SWAP ? t.wrow + half * 128 : t.tok0;
-        const uint8_t* sa = (SWAP ? p.xs + (t.tblk + half) * acols * 512 : p.ws + t.wblk * acols * 512);
-        const uint8_t* sb = (SWAP ? p.ws + t.wblk * acols * 512 : p.xs + t.tblk * acols * 512);
-        const int boxes = SWAP ? 1 : (t.tn + TOK_BOX - 1) / TOK_BOX;
-        const int nb = SWAP && BT > 128 ? (t.nn + 127) >> 7 : 1;          // row blocks of B's scales that exist
-        const int na = half * 128 < t.tn || !SWAP ? 1 : 0;                // and of A's: a pair's second half may have no tokens
-        const uint32_t bytes = A_BYTES + (SWAP ? C::B_BYTES : boxes * TOK_BOX * 128) + (na + nb) * C::SFA;
+        const Tile t = tile_at<BT, C::WT>(p, u, off, base, tiles);
+        const int rows = CG == 2 ? (t.tn + 31) / 32 * 16 : t.tn; // tokens of this CTA
+        const int brow = static_cast<int>(t.tok0) + half * rows, arow = static_cast<int>(t.wrow) + half * 128;
+        const int boxes = rows <= 2 * TOK_BOX ? (rows + TOK_BOX - 1) / TOK_BOX : 0;   // 0: one box of all
+        const uint8_t* sa = p.ws + (t.wblk + half) * acols * 512;
+        const uint8_t* sb = p.xs + t.tblk * acols * 512;
+        // scales that exist: a pair's second half may have no weight rows, its tokens may fill one row block only
+        const int na = half * 128 < t.nn ? 1 : 0, nb = C::NB == 2 ? (t.tn + 127) >> 7 : 1;
+        const uint32_t bytes = A_BYTES + (boxes ? boxes * TOK_BOX * 128 : C::B_BYTES) + (na + nb) * C::SFA;
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
           if (it >= STAGES) mbar_wait(&empty[slot], ((it / STAGES) - 1) & 1, abort_v);
           mbar_arrive_expect_tx(&full[slot], bytes);
-          tma_load_2d(as + slot * A_BYTES, &tm_a, ks * 128, static_cast<int>(arow), &full[slot]);
+          tma_load_2d(as + slot * A_BYTES, &tm_a, ks * 128, arow, &full[slot]);
+          if (!boxes) tma_load_2d(bs + slot * C::B_BYTES, &tm_b, ks * 128, brow, &full[slot]);
           for (int i = 0; i < boxes; ++i)
-            tma_load_2d(bs + slot * C::B_BYTES + i * TOK_BOX * 128, &tm_b, ks * 128, static_cast<int>(brow) + i * TOK_BOX,
-                        &full[slot]);
+            tma_load_2d(bs + slot * C::B_BYTES + i * TOK_BOX * 128, &tm_bs, ks * 128, brow + i * TOK_BOX, &full[slot]);
           if (na) bulk_g2s(sfa + slot * C::SFA, sa + static_cast<int64_t>(ks) * C::SFA, C::SFA, &full[slot]);
           for (int i = 0; i < nb; ++i)
             bulk_g2s(sfb + slot * C::SFB + i * C::SFA, sb + (i * acols * 512 + static_cast<int64_t>(ks) * C::SFA), C::SFA,
@@ -365,8 +347,8 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
       const uint64_t da0 = smem_desc_sw128(smem_u32(as)), db0 = smem_desc_sw128(smem_u32(bs));   // + 16-byte units
       const int last = static_cast<int>(((p.K + 31) / 32 * 32 - (static_cast<int64_t>(p.ksteps) - 1) * 256 + 63) >> 6);
       for (int u = u0; u < units; u += du, ++tc) {
-        const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
-        const int N = SWAP ? BT : (t.tn + 15) / 16 * 16;
+        const Tile t = tile_at<BT, C::WT>(p, u, off, base, tiles);
+        const int N = (t.tn + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const uint32_t id0 = idesc_mx<FMT, CG>(N, 0), id2 = idesc_mx<FMT, CG>(N, 2);
         const uint32_t b = tc % C::ACCS;
         if (tc >= C::ACCS) mbar_wait(&acc_empty[b], ((tc / C::ACCS) - 1) & 1, abort_v);
@@ -377,7 +359,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
           // the warps that stored the scales waited for the stage's copies, so this wait stands for both
           mbar_wait(&sf_full[slot], (it / STAGES) & 1, abort_v);
           tc_fence_after();
-          const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4 + (SWAP ? 0 : t.toff >> 5);
+          const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4 + (t.toff >> 5);
           const uint64_t da = da0 + slot * (A_BYTES >> 4), db = db0 + slot * (C::B_BYTES >> 4);
           const int nk = ks + 1 < p.ksteps ? 4 : last;
 #pragma unroll
@@ -424,51 +406,73 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3, h = (warp - 8) >> 2;                 // lane quarter, part of the columns
     const int rloc = q * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
-    constexpr int HALF = C::COLS;
+    constexpr int COLS = C::COLS;
     uint32_t tc = 0;
     for (int u = u0; u < units; u += du, ++tc) {
-      const Tile t = tile_at<C::TT, C::WT>(p, u, off, base, tiles);
+      const Tile t = tile_at<BT, C::WT>(p, u, off, base, tiles);
       const uint32_t b = tc % C::ACCS;
       mbar_wait(&acc_full[b], (tc / C::ACCS) & 1, abort_v);
       tc_fence_after();
-      const uint32_t d = tmem + lane_addr + b * BT + h * HALF;
-      const int cols = SWAP ? t.nn : t.tn;                       // columns that exist
+      const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BT + h * COLS;
+      const int cl = t.tn - h * COLS < COLS ? t.tn - h * COLS : COLS;   // tokens of this part that exist
       if (S > 1) {                                               // this rank's float32 tile, for the cluster's sum
         float* part = reinterpret_cast<float*>(smem);
-        for (int c0 = 0; c0 < HALF && h * HALF + c0 < cols; c0 += 16) {
+        for (int c0 = 0; c0 < cl; c0 += 16) {
           uint32_t v[16];
           tmem_ld_x16(d + c0, v);
           tc_wait_ld();
-          if (k1 <= k0) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = 0u;
-          }
-          const int c = h * HALF + c0;
-          if (SWAP) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<uint4*>(part + rloc * C::PITCH + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) part[(c + j) * C::PITCH + rloc] = __uint_as_float(v[j]);
-          }
+          for (int j = 0; j < 16; ++j) part[(c0 + j) * C::PITCH + rloc] = k1 > k0 ? __uint_as_float(v[j]) : 0.f;
         }
-      } else if (!SWAP) {
-        const int64_t n = t.n0 + rloc;
-        const bool ok = rloc < t.nn;
-        const float bias = ok ? bias_at(p, t.e * p.N + n) : 0.f;
-        for (int c0 = 0; c0 < HALF && h * HALF + c0 < cols; c0 += 16) {
+        continue;
+      }
+      const int nl = half * 128 + rloc;                          // weight row in the tile
+      const bool ok = nl < t.nn;
+      const float bias = ok ? bias_at(p, t.e * p.N + t.n0 + nl) : 0.f;
+      uint16_t* yc = p.y + (t.tok0 + h * COLS) * p.ldy + t.n0 + nl;
+      if (BT == 256 && !p.acc) {
+        // 64 tokens at a time: packed as bf16, the first leave room for the last, and the accumulator is free (the next
+        // tile's products begin) before those are converted and anything is stored
+        uint32_t o[COLS / 2], v[2][32];
+#pragma unroll
+        for (int g = 0; g < COLS / 64; ++g) {
+          if (64 * g < cl) {
+            tmem_ld_x32(d + 64 * g, v[0]);
+            tmem_ld_x32(d + 64 * g + 32, v[1]);
+            tc_wait_ld();
+          }
+          if (g == COLS / 64 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_first<CG>(&acc_empty[b]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const __nv_bfloat162 bb = __floats2bfloat162_rn(__uint_as_float(v[i][2 * j]) * alpha + bias,
+                                                              __uint_as_float(v[i][2 * j + 1]) * alpha + bias);
+              o[32 * g + 16 * i + j] = *reinterpret_cast<const uint32_t*>(&bb);
+            }
+        }
+        if (!ok) continue;
+#pragma unroll
+        for (int c0 = 0; c0 < COLS; c0 += 16) {
+          if (c0 >= cl) break;
+#pragma unroll
+          for (int c = c0; c < c0 + 16; ++c, yc += p.ldy)
+            if (c < cl) *yc = static_cast<uint16_t>(o[c / 2] >> (16 * (c & 1)));
+        }
+      } else {
+        for (int c0 = 0; c0 < cl; c0 += 16) {
           uint32_t v[16];
           tmem_ld_x16(d + c0, v);
           tc_wait_ld();
-          uint16_t* yc = p.y + (t.tok0 + h * HALF + c0) * p.ldy + n;
-          const int cl = ok ? cols - h * HALF - c0 : 0;
-          if (p.acc) {
+          if (p.acc && ok) {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              if (j < cl)
+              if (c0 + j < cl)
                 v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha + bias +
                                        __uint_as_float(static_cast<uint32_t>(yc[j * p.ldy]) << 16));
           } else {
@@ -477,86 +481,11 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
           }
 #pragma unroll
           for (int j = 0; j < 16; ++j, yc += p.ldy)
-            if (j < cl) *yc = f32_to_bf16_bits_g(__uint_as_float(v[j]));
+            if (ok && c0 + j < cl) *yc = f32_to_bf16_bits_g(__uint_as_float(v[j]));
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[b]);
-      } else {
-        const int64_t m = t.tok0 + half * 128 + rloc;
-        const bool ok = half * 128 + rloc < t.tn;
-        const int cl = cols - h * HALF;                          // columns of the part that exist
-        uint16_t* yr = p.y + m * p.ldy + t.n0 + h * HALF;
-        const uint16_t* br = p.bias ? p.bias + t.e * p.N + t.n0 + h * HALF : nullptr;
-        // 64 columns at a time: packed as bf16, the first leave room for the last, and the accumulator is free (the next tile's
-        // products begin) before those are converted and anything is stored
-        uint32_t o[HALF / 2], v[2][32];
-        auto pack = [&](int g) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[i][j] = __float_as_uint(__uint_as_float(v[i][j]) * alpha);
-            const int c = 64 * g + 32 * i;
-            if (br) add_row(v[i], br + c, cl - c, p.vec & VEC_BIAS);
-            if (p.acc && ok) add_row(v[i], yr + c, cl - c, p.vec & VEC_Y16);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const __nv_bfloat162 bb = __floats2bfloat162_rn(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1]));
-              o[c / 2 + j] = *reinterpret_cast<const uint32_t*>(&bb);
-            }
-          }
-        };
-#pragma unroll
-        for (int g = 0; g < HALF / 64; ++g) {
-          tmem_ld_x32(d + 64 * g, v[0]);
-          tmem_ld_x32(d + 64 * g + 32, v[1]);
-          tc_wait_ld();
-          if (g == HALF / 64 - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_first<CG>(&acc_empty[b]);
-          }
-          pack(g);
-        }
-        if (p.vec & VEC_Y16) {
-          if (ok && (p.vec & VEC_Y32) && cl >= HALF) {           // whole 32-byte sectors
-#pragma unroll
-            for (int i = 0; i < HALF / 16; ++i) stg_v8(yr + 16 * i, o + 8 * i);
-          } else if (ok) {
-#pragma unroll
-            for (int c0 = 0; c0 < HALF; c0 += 8) {
-              if (c0 + 8 <= cl) {
-                *reinterpret_cast<uint4*>(yr + c0) = make_uint4(o[c0 / 2], o[c0 / 2 + 1], o[c0 / 2 + 2], o[c0 / 2 + 3]);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (c0 + j < cl) yr[c0 + j] = static_cast<uint16_t>(o[(c0 + j) / 2] >> (16 * (j & 1)));
-              }
-            }
-          }
-        } else {
-          // rows that are not aligned: 32 x 32 values at a time turned in shared memory, so that a warp stores neighbours of one
-          // row (a lane storing its own row two bytes at a time took 82 us for [1082, 4178], 46 times its bytes' time)
-          const uint32_t mine = smem_u32(turn) + (warp - 8) * 2048;
-          const int rows = t.tn - half * 128 - q * 32;           // rows of this warp that exist
-          uint16_t* yw = p.y + (m - lane) * p.ldy + t.n0 + h * HALF;
-#pragma unroll
-          for (int c0 = 0; c0 < HALF; c0 += 32) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)),
-                           "r"(o[c0 / 2 + 4 * i]), "r"(o[c0 / 2 + 4 * i + 1]), "r"(o[c0 / 2 + 4 * i + 2]), "r"(o[c0 / 2 + 4 * i + 3])
-                           : "memory");
-            __syncwarp();
-            if (c0 + lane < cl) {
-#pragma unroll 8
-              for (int r = 0; r < 32 && r < rows; ++r)
-                yw[r * p.ldy + c0 + lane] = static_cast<uint16_t>(
-                    lds_u16(mine + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2));
-            }
-            __syncwarp();
-          }
-        }
+        if (lane == 0) arrive_first<CG>(&acc_empty[b]);
       }
     }
   }
@@ -566,7 +495,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT, SWAP, CG>::THREADS), 1)
     __syncwarp();
     cluster_sync_all();
     if (u0 < units) {
-      const Tile t = tile_at<C::TT, C::WT>(p, u0, off, base, tiles);
+      const Tile t = tile_at<BT, C::WT>(p, u0, off, base, tiles);
       const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
       const int per = (t.tn * 32 + S - 1) / S, i1 = (rank + 1) * per < t.tn * 32 ? (rank + 1) * per : t.tn * 32;
       for (int i = rank * per + threadIdx.x; i < i1; i += C::THREADS) {
@@ -612,27 +541,27 @@ static bool encode_codes(CUtensorMap* tm, const uint8_t* codes, int64_t rows, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int FMT, int BT, bool SWAP, int CG>
+template <int FMT, int BT>
 static int launch_t(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
-  using C = Cfg<FMT, BT, SWAP, CG>;
+  using C = Cfg<FMT, BT>;
   const int64_t rb = row_bytes(p.K);
   p.ksteps = static_cast<int>((p.K + 255) / 256);
   p.tiles_w = static_cast<int>((p.N + C::WT - 1) / C::WT);
-  p.tiles_t = static_cast<int>((p.M + C::TT - 1) / C::TT);
+  p.tiles_t = static_cast<int>((p.M + BT - 1) / BT);
   // the most units there can be: every group may end in a partly filled tile
-  const int64_t tiles = p.g.G ? p.M / C::TT + (p.g.G < p.M ? p.g.G : p.M) : p.tiles_t;
+  const int64_t tiles = p.g.G ? p.M / BT + (p.g.G < p.M ? p.g.G : p.M) : p.tiles_t;
   const int64_t units = tiles * p.tiles_w;
   if (units > 0x3FFFFFFF / 8) return fail(LB_E_ARG, "%s: too many output tiles", who);
   // K over a cluster while that still fills idle SMs and leaves a rank at least two stages
   int S = 1;
-  if (BT <= 128)
+  if (C::CG == 1)
     while (S < 8 && units * S * 2 <= sms && p.ksteps >= 4 * S) S *= 2;
-  const int cl = CG == 2 ? 2 : S;
-  CUtensorMap tx, tw;
-  if (!encode_codes(&tx, p.xc, p.M, rb, SWAP ? 128 : TOK_BOX) ||
-      !encode_codes(&tw, p.wc, (p.g.G ? p.g.G : 1) * p.N, rb, SWAP ? BT / CG : 128))
+  const int cl = C::CG == 2 ? 2 : S;
+  CUtensorMap tw, tx, txs;
+  if (!encode_codes(&tw, p.wc, (p.g.G ? p.g.G : 1) * p.N, rb, 128) || !encode_codes(&tx, p.xc, p.M, rb, BT / C::CG) ||
+      !encode_codes(&txs, p.xc, p.M, rb, TOK_BOX))
     return fail(LB_E_LAUNCH, "%s: cuTensorMapEncodeTiled failed", who);
-  auto kernel = mx_gemm_kernel<FMT, BT, SWAP, CG>;
+  auto kernel = mx_gemm_kernel<FMT, BT>;
   static std::atomic<uint64_t> ready{0};                          // devices whose limit is set
   int dev = 0;
   cudaGetDevice(&dev);
@@ -655,21 +584,18 @@ static int launch_t(const char* who, GemmMxParams& p, int sms, cudaStream_t st) 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = cl > 1 ? 2 : 1;
-  const CUtensorMap& ta = SWAP ? tx : tw;
-  const CUtensorMap& tb = SWAP ? tw : tx;
-  return launched(cudaLaunchKernelEx(&cfg, kernel, ta, tb, static_cast<const GemmMxParams&>(p)), who);
+  return launched(cudaLaunchKernelEx(&cfg, kernel, tw, tx, txs, static_cast<const GemmMxParams&>(p)), who);
 }
 
 template <int FMT>
 static int launch_f(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
   // tokens per weight: all of them, or what a group has on average
   const int64_t avg = p.g.G ? (p.M + p.g.G - 1) / p.g.G : p.M;
-  if (avg <= 64) return launch_t<FMT, 64, false, 1>(who, p, sms, st);
-  if (avg <= 128) return launch_t<FMT, 128, false, 1>(who, p, sms, st);
+  if (avg <= 64) return launch_t<FMT, 64>(who, p, sms, st);
   // 256 x 256 a pair of SMs once that gives every pair one
   const int64_t tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (tiles >= sms / 2) return launch_t<FMT, 256, true, 2>(who, p, sms, st);
-  return launch_t<FMT, 128, true, 1>(who, p, sms, st);
+  if (avg <= 128 || tiles < sms / 2) return launch_t<FMT, 128>(who, p, sms, st);
+  return launch_t<FMT, 256>(who, p, sms, st);
 }
 
 static int launch_product(const char* who, int fmt, GemmMxParams& p, cudaStream_t st) {
@@ -686,8 +612,6 @@ static int launch_product(const char* who, int fmt, GemmMxParams& p, cudaStream_
   DevInfo* d;
   int r = current(&d);
   if (r) return r;
-  p.vec = (aligned(p.y, 16) && p.ldy % 8 == 0 ? VEC_Y16 : 0) | (aligned(p.y, 32) && p.ldy % 16 == 0 ? VEC_Y32 : 0) |
-          (aligned(p.bias, 16) && p.N % 8 == 0 ? VEC_BIAS : 0);
   return fmt == LB_FMT_MXFP4 ? launch_f<LB_FMT_MXFP4>(who, p, d->sms, st) : launch_f<LB_FMT_NVFP4>(who, p, d->sms, st);
 }
 
@@ -702,7 +626,7 @@ int lb_mx_linear(int fmt, const uint8_t* x_codes, const uint8_t* x_scales, const
                  const uint8_t* w_codes, const uint8_t* w_scales, const float* w_tscale, int64_t N, const void* bias,
                  int accumulate, void* y, int64_t ldy, void* stream) {
   mx::GemmMxParams p{x_codes, x_scales, x_tscale, w_codes, w_scales, w_tscale, static_cast<const uint16_t*>(bias),
-                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {nullptr, 0, 0}, 0, 0, 0, 0};
+                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {nullptr, 0, 0}, 0, 0, 0};
   return mx::launch_product("lb_mx_linear", fmt, p, static_cast<cudaStream_t>(stream));
 }
 
@@ -714,7 +638,7 @@ int lb_mx_linear_grouped(int fmt, const uint8_t* x_codes, const uint8_t* x_scale
   int r = mx::check_groups("lb_mx_linear_grouped", offsets, G, 0, M);
   if (r) return r;
   mx::GemmMxParams p{x_codes, x_scales, x_tscale, w_codes, w_scales, w_tscale, static_cast<const uint16_t*>(bias),
-                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {offsets, static_cast<int>(G), 0}, 0, 0, 0, 0};
+                     static_cast<uint16_t*>(y), M, N, K, ldy, accumulate ? 1 : 0, {offsets, static_cast<int>(G), 0}, 0, 0, 0};
   return mx::launch_product("lb_mx_linear_grouped", fmt, p, static_cast<cudaStream_t>(stream));
 }
 
