@@ -157,14 +157,16 @@ struct Rows {
 
 // The scales of rows that only grow, at one block column: where row r's lie (null: it is in no group).
 struct Walk {
-  uint8_t* col;                                // the column's place in the first row block
-  int64_t block;                               // bytes of a row block
-  int lo, hi;                                  // the current group's rows, and its first row block
-  int64_t blk;
+  const uint8_t* col;                          // the column's place in the first row block
+  uint8_t* here;                               //   and in the current group's first
+  int block;                                   // bytes of a row block (K is below 2^27)
+  int lo, hi;                                  // the current group's rows
   __device__ __forceinline__ Walk(const uint8_t* scales, int64_t c, int64_t acols, const Groups& g)
-      : col(const_cast<uint8_t*>(scales) + (c >> 2) * 512 + (c & 3)), block(acols * 512), lo(0), hi(g.G ? 0 : 0x7FFFFFFF), blk(0) {}
+      : col(scales + (c >> 2) * 512 + (c & 3)), here(const_cast<uint8_t*>(col)), block(static_cast<int>(acols * 512)), lo(0),
+        hi(g.G ? 0 : 0x7FFFFFFF) {}
   __device__ __forceinline__ uint8_t* at(const Groups& g, const int* off, const int* base, int gblocks, int r) {
     if (r >= hi) {
+      int64_t blk;
       if (g.per > 0) {
         const int e = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(g.per));
         lo = e * static_cast<int>(g.per);
@@ -177,9 +179,10 @@ struct Walk {
         hi = off[e + 1];
         blk = base[e];
       }
+      here = const_cast<uint8_t*>(col) + blk * block;
     }
     const int rg = r - lo;
-    return col + (blk + (rg >> 7)) * block + ((rg & 31) * 16 + ((rg >> 5) & 3) * 4);
+    return here + static_cast<int64_t>(rg >> 7) * block + ((rg & 31) * 16 + ((rg >> 5) & 3) * 4);
   }
 };
 
@@ -388,6 +391,7 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
   __shared__ uint32_t turn[8][32 * NW];
   if (cw >= p.K) return;
   Walk walk(p.scales, c, acols, p.g);
+  const uint8_t* const cp = p.codes + c0 / 2;
   struct Packed { uint2 q; uint32_t s; bool in; };
   auto load = [&](int r) {                     // codes and scale byte of a row
     Packed u{make_uint2(0u, 0u), 0u, false};
@@ -395,7 +399,7 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
       const uint8_t* sp = walk.at(p.g, off, base, gblocks, r);
       u.in = sp != nullptr;                    // the same in the whole warp
       if (sp && c0 < p.K) {
-        u.q = *reinterpret_cast<const uint2*>(p.codes + r * rb + c0 / 2);
+        u.q = *reinterpret_cast<const uint2*>(cp + static_cast<int64_t>(r) * static_cast<int>(rb));
         u.s = *sp;
       }
     }
@@ -404,7 +408,9 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
   int r = p.over.first();
   const bool whole = p.vec && c0 + 16 <= p.K;
   Packed next = load(r);
-  for (; r < end; r += step) {
+  const int64_t pitch = p.ldo * ES;
+  char* o = static_cast<char*>(p.out) + r * pitch + c0 * ES;
+  for (; r < end; r += step, o += step * pitch) {
     const Packed now = next;
     next = load(r + step);
     if (!now.in) continue;
@@ -446,7 +452,6 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
         }
       }
     }
-    char* o = static_cast<char*>(p.out) + (r * p.ldo + c0) * ES;
     if (p.vec) {
       if (whole) {
 #pragma unroll
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(256, DEQUANT_BLOCKS) dequant_kernel_mx(const D
       for (int i = 0; i < NW; ++i) tile[lane * NW + ((i + lane) & (NW - 1))] = u[i];
       __syncwarp();
       const int n = static_cast<int>(p.K - cw < 512 ? p.K - cw : 512);
-      char* ow = static_cast<char*>(p.out) + (r * p.ldo + cw) * ES;
+      char* ow = o - lane * 16 * ES;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int j = 32 * i + lane, l = j >> 4;               // value j of the warp's 512 is with lane l
