@@ -4,21 +4,24 @@
 // The tensor cores multiply the codes and the block scales as they are stored (tcgen05.mma, kind mxf4 / mxf4nvf4 with
 // block_scale), 64 values of K an instruction, float32 accumulators in tensor memory; nothing is expanded.
 // A stage is 256 values of K: 128 bytes of codes a row (one 128-byte swizzled TMA row) of the two operand tiles and their
-// scale atoms.  Four warps move the atoms into tensor memory (tcgen05.st; the four copies in the lane quarters that the
-// products want are one store of each warp), a slot per stage, so a slot is not written again before the products
-// that read it are done (the stage's own `empty` barrier).  As tcgen05.cp they cost the tensor pipe about 45 cycles
-// an atom: with 12 atoms against 512 cycles of nvfp4 products a stage that was the bound.
+// scale atoms, which go to tensor memory, a slot per stage, so a slot is not written again before the products that
+// read it are done (the stage's own `empty` barrier).  Four warps store them there (tcgen05.st; the four copies in the lane
+// quarters that the products want are one store of each warp): with few tokens that keeps them out of the thread that issues the
+// products, which has to be quick ([64 x 28672 x 8192] nvfp4 50 -> 40 us against copies by that thread).  A pair's products
+// take longer than their issue, and there tcgen05.cp, which reads shared memory once where the warps read it four times,
+// is the better one under the power limit ([2048 x 28672 x 8192] mxfp4 224 -> 218 us a pass).
 //
 // A (the rows of the accumulator, tensor memory's lanes) is 128 weight rows, B (its columns) up to BT = 64, 128 or 256 tokens; a
 // tile with fewer tokens multiplies only those (rounded up to 16, a pair 32), so a ragged group's last tile costs what it holds.
 // Weights on the lanes also make a warp's store 32 neighbours of a row of y, whatever its alignment.
 //   BT = 256   a pair of CTAs (cta_group::2) on 256 weight rows x 256 tokens: each loads its own 128 weight rows and half of
 //              the tokens, so a product needs 16 KB of codes from L2 for every 128 x 256 outputs and 256 of K, not 24
-// What bounds a pair's stage is the shared memory: 35 KB (mxfp4) or 39 KB (nvfp4) written by TMA, 32 KB read by the products, 12 or
-// 24 KB by the four warps that take the scales, at 128 bytes a cycle 620 or 740 cycles against 512 of products.
+// What bounds a pair: the tensor pipe is busy 72 % of the time ([2048 x 28672 x 8192], 162 us at 1.7 GHz); the rest is the
+// accumulator's change of hands (2100 cycles a tile) and, run without a pause, the power limit (1.5 GHz).  What bounds few
+// tokens is HBM and the start: [64 x 28672 x 8192] reads its 132 MB at 5 TB/s.
 //
-// Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales, 8.. epilogue (4 or 8 warps; warp w reads lanes
-// 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
+// Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales (in a pair 2 passes word of its CTA's copies on), then
+// 4 or 8 of the epilogue (warp w reads lanes 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
 // takes it into registers at once and converts and stores while the next tile's products run.
 //
 // Few units (decode, small layers): a cluster of S CTAs splits K; each leaves its float32 tile in its own shared
@@ -67,13 +70,20 @@ struct Cfg {
   static constexpr int PITCH = 132;                              // floats of a token's row in the cluster's tile (128 outputs)
   static_assert(CG == 2 || STAGES * STAGE >= BT * PITCH * 4, "the cluster's tile reuses the stages");
   static constexpr int EW = 4 * CG;                              // epilogue warps
-  static constexpr int THREADS = (8 + EW) * 32;
+  static constexpr int EPI = CG == 2 ? 4 : 8;                    // the first of them
+  static constexpr int THREADS = (EPI + EW) * 32;
   static constexpr int COLS = BT / CG;                           // columns of an epilogue warp
   static constexpr int LISTS = BT == 128 ? 2 : 3;                // words per group: off, base, (token tiles)
   static int smem(int G) { return 1024 + STAGES * STAGE + 256 + (G ? LISTS * (G + 1) * 4 : 0); }
   static_assert(1024 + STAGES * STAGE + 256 + LISTS * (LB_MX_MAX_GROUPS + 1) * 4 <= SMEM_MAX, "shared memory");
 };
 
+// One scale atom from shared memory (32 rows of 16 bytes, 8-row pieces 128 bytes apart, no swizzle) to all lane quarters, in
+// both CTAs of a pair.
+__device__ __forceinline__ void tc_cp_scales_pair(uint32_t tmem, uint32_t smem) {
+  const uint64_t desc = static_cast<uint64_t>((smem >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
 template <int FMT, int CG>
 __device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                           uint32_t accumulate) {
@@ -248,7 +258,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
   uint8_t* sfb = sfa + STAGES * C::SFA;
   uint64_t* full = reinterpret_cast<uint64_t*>(sfb + STAGES * C::SFB);
   uint64_t* empty = full + STAGES;
-  uint64_t* sf_full = empty + STAGES;                            // a stage's scales are in tensor memory
+  uint64_t* sf_full = empty + STAGES;                            // a stage's scales are in tensor memory (pair: both CTAs' copies landed)
   uint64_t* acc_full = sf_full + STAGES;                         // [ACCS]
   uint64_t* acc_empty = acc_full + 2;                            // [ACCS]
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
@@ -263,7 +273,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&sf_full[s], 4 * CG);
+      mbar_init(&sf_full[s], CG == 2 ? 2 : 4);
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -356,11 +366,21 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
         const uint32_t d = tmem + b * BT;
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
-          // the warps that stored the scales waited for the stage's copies, so this wait stands for both
+          // those who arrive here waited for the stage's copies, so this wait stands for both
           mbar_wait(&sf_full[slot], (it / STAGES) & 1, abort_v);
           tc_fence_after();
           const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4 + (t.toff >> 5);
           const uint64_t da = da0 + slot * (A_BYTES >> 4), db = db0 + slot * (C::B_BYTES >> 4);
+          if constexpr (CG == 2) {                               // columns [K atom][row block][4]
+            const uint32_t fa = smem_u32(sfa + slot * C::SFA), fb = smem_u32(sfb + slot * C::SFB);
+#pragma unroll
+            for (int a = 0; a < AT; ++a) {
+              tc_cp_scales_pair(ca + a * 4, fa + a * 512);
+#pragma unroll
+              for (int i = 0; i < C::NB; ++i)
+                tc_cp_scales_pair(ca + AT * 4 + a * (4 * C::NB) + i * 4, fb + i * C::SFA + a * 512);
+            }
+          }
           const int nk = ks + 1 < p.ksteps ? 4 : last;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
@@ -374,37 +394,48 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
         tc_commit_all<CG>(&acc_full[b]);
       }
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (CG == 2 ? warp == 2 : warp >= 4 && warp < 8) {
     // ------------------------------------------------------------------ scales into tensor memory
-    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    uint32_t it = 0;
-    for (int u = u0; u < units; u += du) {
-      for (int ks = k0; ks < k1; ++ks, ++it) {
-        const uint32_t slot = it % STAGES;
-        mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
-        const uint32_t ca = tmem + lane_addr + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
-        const uint32_t fa = smem_u32(sfa + slot * C::SFA) + lane * 16, fb = smem_u32(sfb + slot * C::SFB) + lane * 16;
-        uint4 v[AT * (1 + C::NB)];
+    if constexpr (CG == 2) {                                     // the MMA thread copies them: pass word of this CTA's copies on
+      if (elect_one()) {
+        uint32_t it = 0;
+        for (int u = u0; u < units; u += du)
+          for (int ks = k0; ks < k1; ++ks, ++it) {
+            mbar_wait(&full[it % STAGES], (it / STAGES) & 1, abort_v);
+            arrive_first<CG>(&sf_full[it % STAGES]);
+          }
+      }
+    } else {
+      const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      uint32_t it = 0;
+      for (int u = u0; u < units; u += du) {
+        for (int ks = k0; ks < k1; ++ks, ++it) {
+          const uint32_t slot = it % STAGES;
+          mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
+          const uint32_t ca = tmem + lane_addr + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
+          const uint32_t fa = smem_u32(sfa + slot * C::SFA) + lane * 16, fb = smem_u32(sfb + slot * C::SFB) + lane * 16;
+          uint4 v[AT * (1 + C::NB)];
 #pragma unroll
-        for (int a = 0; a < AT; ++a) {
-          v[a] = lds_v4(fa + a * 512);
+          for (int a = 0; a < AT; ++a) {
+            v[a] = lds_v4(fa + a * 512);
 #pragma unroll
-          for (int i = 0; i < C::NB; ++i) v[AT + a * C::NB + i] = lds_v4(fb + i * C::SFA + a * 512);
+            for (int i = 0; i < C::NB; ++i) v[AT + a * C::NB + i] = lds_v4(fb + i * C::SFA + a * 512);
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int a = 0; a < AT; ++a) tmem_st_x4(ca + a * 4, v[a]);
+#pragma unroll
+          for (int a = 0; a < AT * C::NB; ++a) tmem_st_x4(cb + a * 4, v[AT + a]);   // columns [K atom][row block][4]
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sf_full[slot]);
         }
-        tc_fence_after();
-#pragma unroll
-        for (int a = 0; a < AT; ++a) tmem_st_x4(ca + a * 4, v[a]);
-#pragma unroll
-        for (int a = 0; a < AT * C::NB; ++a) tmem_st_x4(cb + a * 4, v[AT + a]);   // columns [K atom][row block][4]
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_first<CG>(&sf_full[slot]);
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= C::EPI) {
     // ------------------------------------------------------------------ epilogue
-    const int q = warp & 3, h = (warp - 8) >> 2;                 // lane quarter, part of the columns
+    const int q = warp & 3, h = (warp - C::EPI) >> 2;            // lane quarter, part of the columns
     const int rloc = q * 32 + lane;
     const float alpha = (p.xt ? *p.xt : 1.f) * (p.wt ? *p.wt : 1.f);
     constexpr int COLS = C::COLS;
