@@ -16,9 +16,9 @@
 // Weights on the lanes also make a warp's store 32 neighbours of a row of y, whatever its alignment.
 //   BT = 256   a pair of CTAs (cta_group::2) on 256 weight rows x 256 tokens: each loads its own 128 weight rows and half of
 //              the tokens, so a product needs 16 KB of codes from L2 for every 128 x 256 outputs and 256 of K, not 24
-// What bounds a pair: the tensor pipe is busy 72 % of the time ([2048 x 28672 x 8192], 162 us at 1.7 GHz); the rest is the
-// accumulator's change of hands (2100 cycles a tile) and, run without a pause, the power limit (1.5 GHz).  What bounds few
-// tokens is HBM and the start: [64 x 28672 x 8192] reads its 132 MB at 5 TB/s.
+// What bounds a pair: the tensor pipe is busy 85 % of its time ([2048 x 28672 x 8192] mxfp4, 167 us, 5770 TFLOP/s); the rest is
+// the accumulator's change of hands (about 2100 cycles a tile) and, run without a pause, the power limit.  What bounds few tokens
+// is HBM and the start: [64 x 28672 x 8192] nvfp4 reads its 132 MB at 5 TB/s.
 //
 // Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales (in a pair 2 passes word of its CTA's copies on), then
 // 4 or 8 of the epilogue (warp w reads lanes 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
