@@ -15,20 +15,21 @@
 // tile with fewer tokens multiplies only those (rounded up to 16, a pair 32), so a ragged group's last tile costs what it holds.
 // Weights on the lanes also make a warp's store 32 neighbours of a row of y, whatever its alignment.
 //   BT = 256   a pair of CTAs (cta_group::2) on 256 weight rows x 256 tokens: each loads its own 128 weight rows and half of
-//              the tokens, so a product needs 16 KB of codes from L2 for every 128 x 256 outputs and 256 of K, not 24
+//              the tokens, so 128 x 256 outputs need 32 KB of codes from L2 for 256 of K, not 48
 // What bounds a pair: the tensor pipe is busy 85 % of its time ([2048 x 28672 x 8192] mxfp4, 167 us, 5770 TFLOP/s); the rest is
 // the accumulator's change of hands (about 2100 cycles a tile) and, run without a pause, the power limit.  What bounds few tokens
 // is HBM and the start: [64 x 28672 x 8192] nvfp4 reads its 132 MB at 5 TB/s.
 //
 // Roles: warp 0 TMA, 1 MMA (in a pair the first CTA's only), 4..7 scales (in a pair 2 passes word of its CTA's copies on), then
-// 4 or 8 of the epilogue (warp w reads lanes 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator only (256 columns + the stages' scales): the epilogue
-// takes it into registers at once and converts and stores while the next tile's products run.
+// 4 or 8 of the epilogue (warp w reads lanes 32 (w % 4) .. + 31).  BT = 256 leaves tensor memory for one accumulator
+// only (256 columns + the stages' scales): the epilogue takes it into registers and stores while the next tile's products run.
 //
 // Few units (decode, small layers): a cluster of S CTAs splits K; each leaves its float32 tile in its own shared
 // memory and every CTA adds its share of the outputs over the cluster in rank order: one launch, no workspace, the
 // same bits every time.
 //
-// All mbarrier waits are bounded (lb::mbar_wait); a timeout sets the device error word and the CTA drains.
+// All mbarrier waits are bounded (lb::mbar_wait).  A wait that gives up sets the device error word; every role then leaves its
+// loops, the copies and products already issued are given time to land, and the CTA frees its tensor memory and ends.
 #include "lb_mx.cuh"
 #include "lb_tmap.h"
 #include "lb_kernels.h"
@@ -325,7 +326,8 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
     // ------------------------------------------------------------------ TMA producer
     if (elect_one()) {
       uint32_t it = 0;
-      for (int u = u0; u < units; u += du) {
+      bool alive = true;
+      for (int u = u0; u < units && alive; u += du) {
         const Tile t = tile_at<BT, C::WT>(p, u, off, base, tiles);
         const int rows = CG == 2 ? (t.tn + 31) / 32 * 16 : t.tn; // tokens of this CTA
         const int brow = static_cast<int>(t.tok0) + half * rows, arow = static_cast<int>(t.wrow) + half * 128;
@@ -337,7 +339,10 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
         const uint32_t bytes = A_BYTES + (boxes ? boxes * TOK_BOX * 128 : C::B_BYTES) + (na + nb) * C::SFA;
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
-          if (it >= STAGES) mbar_wait(&empty[slot], ((it / STAGES) - 1) & 1, abort_v);
+          if (it >= STAGES && !mbar_wait(&empty[slot], ((it / STAGES) - 1) & 1, abort_v)) {
+            alive = false;
+            break;
+          }
           mbar_arrive_expect_tx(&full[slot], bytes);
           tma_load_2d(as + slot * A_BYTES, &tm_a, ks * 128, arow, &full[slot]);
           if (!boxes) tma_load_2d(bs + slot * C::B_BYTES, &tm_b, ks * 128, brow, &full[slot]);
@@ -349,6 +354,8 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
                      &full[slot]);
         }
       }
+      if (*abort_v)                                              // copies in flight land before the CTA ends
+        for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, abort_v);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
@@ -356,18 +363,22 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
       uint32_t it = 0, tc = 0;
       const uint64_t da0 = smem_desc_sw128(smem_u32(as)), db0 = smem_desc_sw128(smem_u32(bs));   // + 16-byte units
       const int last = static_cast<int>(((p.K + 31) / 32 * 32 - (static_cast<int64_t>(p.ksteps) - 1) * 256 + 63) >> 6);
-      for (int u = u0; u < units; u += du, ++tc) {
+      bool alive = true;
+      for (int u = u0; u < units && alive; u += du, ++tc) {
         const Tile t = tile_at<BT, C::WT>(p, u, off, base, tiles);
         const int N = (t.tn + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const uint32_t id0 = idesc_mx<FMT, CG>(N, 0), id2 = idesc_mx<FMT, CG>(N, 2);
         const uint32_t b = tc % C::ACCS;
-        if (tc >= C::ACCS) mbar_wait(&acc_empty[b], ((tc / C::ACCS) - 1) & 1, abort_v);
+        if (tc >= C::ACCS && !mbar_wait(&acc_empty[b], ((tc / C::ACCS) - 1) & 1, abort_v)) break;
         tc_fence_after();
         const uint32_t d = tmem + b * BT;
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
           // those who arrive here waited for the stage's copies, so this wait stands for both
-          mbar_wait(&sf_full[slot], (it / STAGES) & 1, abort_v);
+          if (!mbar_wait(&sf_full[slot], (it / STAGES) & 1, abort_v)) {
+            alive = false;
+            break;
+          }
           tc_fence_after();
           const uint32_t ca = tmem + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4 + (t.toff >> 5);
           const uint64_t da = da0 + slot * (A_BYTES >> 4), db = db0 + slot * (C::B_BYTES >> 4);
@@ -391,7 +402,12 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
           }
           tc_commit_all<CG>(&empty[slot]);
         }
-        tc_commit_all<CG>(&acc_full[b]);
+        if (alive) tc_commit_all<CG>(&acc_full[b]);
+      }
+      if (*abort_v) {                                            // products in flight end before tensor memory is freed
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 200000u) {
+        }
       }
     }
   } else if (CG == 2 ? warp == 2 : warp >= 4 && warp < 8) {
@@ -399,19 +415,22 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
     if constexpr (CG == 2) {                                     // the MMA thread copies them: pass word of this CTA's copies on
       if (elect_one()) {
         uint32_t it = 0;
-        for (int u = u0; u < units; u += du)
-          for (int ks = k0; ks < k1; ++ks, ++it) {
-            mbar_wait(&full[it % STAGES], (it / STAGES) & 1, abort_v);
-            arrive_first<CG>(&sf_full[it % STAGES]);
+        bool alive = true;
+        for (int u = u0; u < units && alive; u += du)
+          for (int ks = k0; ks < k1 && alive; ++ks, ++it) {
+            alive = mbar_wait(&full[it % STAGES], (it / STAGES) & 1, abort_v);
+            if (alive) arrive_first<CG>(&sf_full[it % STAGES]);
           }
       }
     } else {
       const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
       uint32_t it = 0;
-      for (int u = u0; u < units; u += du) {
+      bool alive = true;
+      for (int u = u0; u < units && alive; u += du) {
         for (int ks = k0; ks < k1; ++ks, ++it) {
           const uint32_t slot = it % STAGES;
-          mbar_wait(&full[slot], (it / STAGES) & 1, abort_v);
+          alive = __all_sync(0xffffffffu, mbar_wait(&full[slot], (it / STAGES) & 1, abort_v));
+          if (!alive) break;
           const uint32_t ca = tmem + lane_addr + C::ACCS * BT + slot * C::SF_COLS, cb = ca + AT * 4;
           const uint32_t fa = smem_u32(sfa + slot * C::SFA) + lane * 16, fb = smem_u32(sfb + slot * C::SFB) + lane * 16;
           uint4 v[AT * (1 + C::NB)];
@@ -443,7 +462,7 @@ __global__ void __launch_bounds__((Cfg<FMT, BT>::THREADS), 1)
     for (int u = u0; u < units; u += du, ++tc) {
       const Tile t = tile_at<BT, C::WT>(p, u, off, base, tiles);
       const uint32_t b = tc % C::ACCS;
-      mbar_wait(&acc_full[b], (tc / C::ACCS) & 1, abort_v);
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (tc / C::ACCS) & 1, abort_v))) break;
       tc_fence_after();
       const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * BT + h * COLS;
       const int cl = t.tn - h * COLS < COLS ? t.tn - h * COLS : COLS;   // tokens of this part that exist
