@@ -602,7 +602,8 @@ static int launch_t(const char* who, GemmMxParams& p, int sms, cudaStream_t st) 
   const int64_t tiles = p.g.G ? p.M / BT + (p.g.G < p.M ? p.g.G : p.M) : p.tiles_t;
   const int64_t units = tiles * p.tiles_w;
   if (units > 0x3FFFFFFF / 8) return fail(LB_E_ARG, "%s: too many output tiles", who);
-  // K over a cluster while that still fills idle SMs and leaves a rank at least two stages
+  // K over a cluster while that still fills idle SMs and leaves a rank at least two stages ([1 x 4096 x 4096] 6.5 us, unsplit 7.6;
+  // [4 x 4096 x 11008] 8.3, unsplit 13.6)
   int S = 1;
   if (C::CG == 1)
     while (S < 8 && units * S * 2 <= sms && p.ksteps >= 4 * S) S *= 2;
@@ -639,7 +640,11 @@ static int launch_t(const char* who, GemmMxParams& p, int sms, cudaStream_t st) 
 
 template <int FMT>
 static int launch_f(const char* who, GemmMxParams& p, int sms, cudaStream_t st) {
-  // tokens per weight: all of them, or what a group has on average
+  // By the tokens of a weight (all of them, or what a group has on average): the 64-token tile leaves shared memory for 7 or 8
+  // stages of the weight stream ([48 x 11008 x 4096] nvfp4 9.8 us, with 128-token tiles 11.9; [128 x 11008 x 4096] 11.6 with
+  // 128-token tiles, 14.5 with 64); pairs halve the traffic of the tokens ([2048 x 12288 x 4096] nvfp4 52 us, without 65), but
+  // a pair with half a tile of tokens pays for the whole of its handshakes (4000 rows over 32 experts of [2816, 2048] 36 us
+  // with 128-token tiles, 44 with pairs).
   const int64_t avg = p.g.G ? (p.M + p.g.G - 1) / p.g.G : p.M;
   if (avg <= 64) return launch_t<FMT, 64>(who, p, sms, st);
   // 256 x 256 a pair of SMs once that gives every pair one
