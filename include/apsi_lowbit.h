@@ -290,7 +290,8 @@ int64_t lb_mx_scale_bytes(int fmt, int64_t R, int64_t K, int64_t G, int64_t per)
  * e2m1(x' / s); t = *tensor_scale (device, positive), or with tensor_scale == NULL the smallest power of two with
  * max|x| / t <= 448 * 6 over all finite values of x, found in a pass of its own and written to auto_scale[0] (device,
  * 1 + LB_MX_PARTIALS floats).  Nearest, ties to the even code, saturating; a block with a NaN or an infinity gets a
- * NaN scale.  Rows of no group are not written.  codes and scales 16-byte aligned. */
+ * NaN scale.  Rows of no group are not written.  codes and scales 16-byte aligned.  At most 2^31 - 256 rows of 2^27 - 1
+ * values. */
 int lb_mx_quant(int fmt, const void* x, int x_dtype, int64_t Rin, int64_t K, int64_t ldx, const int* rows, int64_t R,
                 const int* offsets, int64_t G, int64_t per, const float* tensor_scale, float* auto_scale, uint8_t* codes,
                 uint8_t* scales, void* stream);

@@ -188,7 +188,8 @@ def product_case(mx, fmt, M, N, K, seed=0, **kw):
 
 SHAPES = [(1, 128, 256), (1, 1, 32), (1, 17, 1), (2, 300, 31), (3, 257, 100), (16, 512, 1024), (17, 130, 288), (33, 4096, 4096),
           (64, 1000, 8192), (65, 256, 544), (100, 11008, 320), (128, 640, 2048), (129, 129, 129), (200, 333, 4096),
-          (257, 513, 777), (300, 8200, 160), (1000, 4096, 96), (2048, 5000, 512), (1, 28672, 8192), (2300, 300, 64)]
+          (257, 513, 777), (300, 8200, 160), (1000, 4096, 96), (2048, 5000, 512), (1, 28672, 8192), (2300, 300, 64),
+          (5, 600, 8448), (2, 100, 70000), (257, 20000, 512)]
 
 
 @pytest.mark.parametrize("fmt", FMTS)
