@@ -190,18 +190,21 @@ def quantize(x, fmt, tensor_scale=None, rows=None, offsets=None):
         G = _index(offsets, "offsets", dev) - 1
         if not 0 < G <= MX_MAX_GROUPS:
             raise _err(f"offsets must hold 2 to {MX_MAX_GROUPS + 1} values, got {G + 1}")
-    t = _tensor_scale(fmt, tensor_scale, dev)
-    nc, ns = R * _row_bytes(K), _scale_bytes(fmt, R, K, G, per)
+    t = None if tensor_scale is None and fmt == "mxfp4" else _tensor_scale(fmt, tensor_scale, dev)
+    nc, ns = R * ((K + 31) // 32 * 16), _scale_bytes(fmt, R, K, G, per)
     tail = 4 * (1 + MX_PARTIALS) if t is None and fmt == "nvfp4" else 0
     buf = x.new_empty(nc + ns + tail, dtype=torch.uint8)
     codes = buf.data_ptr()
-    found = codes + nc + ns if tail else None
-    if tail and R == 0:
-        buf[nc + ns:].view(torch.float32)[0] = 1.0
-    _launch(dev, "lb_mx_quant", f, x.data_ptr(), dt, R_in, K, ldx, _ptr(rows), R, _ptr(offsets), G, per, _ptr(t), found, codes,
-            codes + nc)
-    return MxTensor(fmt, shape, R, buf, codes, codes + nc, found if t is None else t.data_ptr(), offsets,
-                    None if t is None else (None, None, t), tail)
+    scale = found = None
+    if t is not None:
+        scale = t.data_ptr()
+    elif tail:
+        found = codes + nc + ns
+        if R == 0:
+            buf[nc + ns:].view(torch.float32)[0] = 1.0
+    _launch(dev, "lb_mx_quant", f, x.data_ptr(), dt, R_in, K, ldx, None if rows is None else rows.data_ptr(), R,
+            None if offsets is None else offsets.data_ptr(), G, per, scale, found, codes, codes + nc)
+    return MxTensor(fmt, shape, R, buf, codes, codes + nc, scale or found, offsets, None if t is None else (None, None, t), tail)
 
 
 def dequantize(q, dtype=torch.float32):
